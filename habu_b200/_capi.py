@@ -15,7 +15,7 @@ HB_OK, HB_ERR_INVALID, HB_ERR_NOT_FOUND, HB_ERR_DUPLICATE, HB_ERR_CUDA, HB_ERR_N
     HB_ERR_TIMEOUT, HB_ERR_UNSUPPORTED, HB_ERR_NOMEM = range(9)
 STATUS_NAMES = ["OK", "Invalid", "Not_found", "Duplicate", "Cuda", "Nccl", "Timeout",
                 "Unsupported", "No_memory"]
-HB_F32, HB_BF16, HB_I32 = 0, 1, 2
+HB_F32, HB_BF16, HB_I32, HB_E4M3 = 0, 1, 2, 3
 HB_EPI_NONE, HB_EPI_GELU, HB_EPI_SWIGLU, HB_EPI_RESIDUAL = 0, 1, 2, 3
 HB_AR_AUTO, HB_AR_NCCL, HB_AR_P2P, HB_AR_NVLS = 0, 1, 2, 3
 HB_OP_MATMUL, HB_OP_ATTENTION = 0, 1
@@ -100,6 +100,10 @@ def load() -> C.CDLL:
         "hb_mse": [vp, vp, vp, vp, vp, i64],
         "hb_adam_step": [vp, vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, i64, f32],
         "hb_adam_step_async": [vp, vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, i64, f32],
+        "hb_quantize": [vp, T, T, T, i32],
+        "hb_rmsnorm_quant": [vp, T, vp, T, T, T, f32],
+        "hb_swiglu_quant": [vp, T, T, T],
+        "hb_matmul_scaled": [vp, T, T, T, T, T, C.POINTER(hb_matmul_opts)],
         "hb_comm_unique_id": [vp],
         "hb_comm_init_rank": [vp, i32, i32, vp],
         "hb_comm_destroy": [vp],

@@ -15,7 +15,7 @@
 
 // Device status word layout (int32[4]): [0] first error code, [1] kernel tag that
 // reported it, [2] detail (e.g. which wait), [3] reserved.
-enum { HB_KTAG_GEMM = 1, HB_KTAG_ATTN = 2, HB_KTAG_ALLREDUCE = 3, HB_KTAG_SPLITK = 4, HB_KTAG_DECODE = 5 };
+enum { HB_KTAG_GEMM = 1, HB_KTAG_ATTN = 2, HB_KTAG_ALLREDUCE = 3, HB_KTAG_SPLITK = 4, HB_KTAG_DECODE = 5, HB_KTAG_SCALED = 6 };
 
 // Scratch slots: kernel workspace (split-K partials), host-call staging, autotune operands.
 enum { HB_SCRATCH_WORKSPACE = 0, HB_SCRATCH_STAGING = 1, HB_SCRATCH_TUNE = 2, HB_SCRATCH_REDUCE = 3, HB_SCRATCH_DECODE = 4, HB_NUM_SCRATCH = 5 };
@@ -112,6 +112,20 @@ inline cudaError_t hb_launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// Makes the context's device current for the scope of an entry point and puts the caller's back.
+struct hb_device_guard {
+  int before = -1, mine = -1;
+  explicit hb_device_guard(const hb_ctx* ctx) : mine(ctx->device) {
+    if (cudaGetDevice(&before) != cudaSuccess) { cudaGetLastError(); before = -1; }
+    if (before != mine) cudaSetDevice(mine);
+  }
+  ~hb_device_guard() {
+    if (before >= 0 && before != mine) cudaSetDevice(before);
+  }
+  hb_device_guard(const hb_device_guard&) = delete;
+  hb_device_guard& operator=(const hb_device_guard&) = delete;
+};
+
 hb_status hb_fail(hb_ctx* ctx, hb_status code, const char* fmt, ...);
 hb_status hb_check_cuda(hb_ctx* ctx, cudaError_t e, const char* what);
 #define HB_CUDA(ctx, call)                                        \
@@ -119,6 +133,8 @@ hb_status hb_check_cuda(hb_ctx* ctx, cudaError_t e, const char* what);
     cudaError_t e__ = (call);                                     \
     if (e__ != cudaSuccess) return hb_check_cuda(ctx, e__, #call); \
   } while (0)
+// Scales of a quantised matrix: fp32 [d0, d1], every element with a place of its own.
+hb_status hb_check_scales(hb_ctx* ctx, const char* op, const hb_tensor* s, int64_t d0, int64_t d1);
 // Drains every stream the context may have queued work on (before freeing its memory).
 hb_status hb_quiesce(hb_ctx* ctx);
 // Grow-only scratch buffer `slot` on the context's device.

@@ -13,18 +13,18 @@ host-side sources and destinations of explicit uploads and downloads.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Optional, Sequence
 
 import numpy as np
 
 from . import _capi
-from ._capi import (HB_AR_AUTO, HB_AR_NCCL, HB_AR_NVLS, HB_AR_P2P, HB_BF16, HB_EPI_GELU, HB_EPI_NONE,
+from ._capi import (HB_AR_AUTO, HB_AR_NCCL, HB_AR_NVLS, HB_AR_P2P, HB_BF16, HB_E4M3, HB_EPI_GELU, HB_EPI_NONE,
                     HB_EPI_RESIDUAL, HB_EPI_SWIGLU, HB_F32, HB_I32, HB_OP_MATMUL,
                     HB_TUNE_CACHED, HB_TUNE_SEARCH)
 
 _lib = _capi.load()
-_ELEM = {HB_F32: 4, HB_BF16: 2, HB_I32: 4}
+_ELEM = {HB_F32: 4, HB_BF16: 2, HB_I32: 4, HB_E4M3: 1}
 
 
 class HabuError(RuntimeError):
@@ -41,6 +41,7 @@ class Tensor:
     shape: tuple
     stride: tuple
     owner: object = None
+    _c: object = field(default=None, init=False, repr=False, compare=False)
 
     @property
     def nbytes(self) -> int:
@@ -55,14 +56,13 @@ class Tensor:
         return Tensor(self.ptr, self.dtype, self.shape[::-1], self.stride[::-1], self.owner)
 
     def c(self) -> _capi.hb_tensor:
-        t = _capi.hb_tensor()
-        t.ptr = self.ptr
-        t.dtype = self.dtype
-        t.rank = len(self.shape)
-        for i, (s, st) in enumerate(zip(self.shape, self.stride)):
-            t.shape[i] = s
-            t.stride[i] = st
-        return t
+        """The C view.  Building one costs more host time than a small launch, so it is kept until
+        a field it was made from changes."""
+        key = (self.ptr, self.dtype, self.shape, self.stride)
+        if self._c is None or self._c[0] != key:
+            self._c = key, _capi.hb_tensor(self.ptr, self.dtype, len(self.shape), (C.c_int64 * 4)(*self.shape),
+                                           (C.c_int64 * 4)(*self.stride))
+        return self._c[1]
 
 
 def f32_to_bf16_bits(x: np.ndarray) -> np.ndarray:
@@ -145,18 +145,18 @@ class Context:
 
     def upload(self, host: np.ndarray, dtype: Optional[int] = None) -> Tensor:
         """Copy a C-contiguous host array to a new device tensor.  uint16 arrays are
-        bf16 bit patterns, float32 -> HB_F32, int32 -> HB_I32."""
+        bf16 bit patterns, uint8 arrays e4m3 bit patterns, float32 -> HB_F32, int32 -> HB_I32."""
         host = np.ascontiguousarray(host)
         if dtype is None:
             dtype = {np.dtype(np.uint16): HB_BF16, np.dtype(np.float32): HB_F32,
-                     np.dtype(np.int32): HB_I32}[host.dtype]
+                     np.dtype(np.int32): HB_I32, np.dtype(np.uint8): HB_E4M3}[host.dtype]
         t = self.empty(host.shape, dtype)
         self._check(_lib.hb_upload(self._h, C.c_void_p(t.ptr), host.ctypes.data_as(C.c_void_p), host.nbytes))
         self.sync()
         return t
 
     def download(self, t: Tensor) -> np.ndarray:
-        np_dtype = {HB_BF16: np.uint16, HB_F32: np.float32, HB_I32: np.int32}[t.dtype]
+        np_dtype = {HB_BF16: np.uint16, HB_F32: np.float32, HB_I32: np.int32, HB_E4M3: np.uint8}[t.dtype]
         assert t.stride == _contig(t.shape), "download needs a contiguous tensor"
         out = np.empty(t.shape, np_dtype)
         self._check(_lib.hb_download(self._h, out.ctypes.data_as(C.c_void_p), C.c_void_p(t.ptr), out.nbytes))
@@ -303,6 +303,59 @@ class Context:
         rows, cols = x.shape
         out = self.empty((rows,), HB_I32)
         self._check(_lib.hb_argmax(self._h, x.ptr, out.ptr, rows, cols))
+        return out
+
+    # -- 8-bit path -----------------------------------------------------------------
+    def empty_quantised(self, rows: int, cols: int, block_rows: int = 1):
+        """A (q, scale) pair for [rows, cols]: e4m3 rows padded to a multiple of 16 bytes (what
+        the scaled product loads) and one fp32 scale per 128 values or 128 x 128 block."""
+        q = self.empty((rows, (cols + 15) // 16 * 16), HB_E4M3)
+        q.shape = (rows, cols)
+        return q, self.empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), HB_F32)
+
+    def quantize(self, x: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None, block_rows: int = 1):
+        """x [rows, cols] bf16 or fp32 -> (q e4m3 [rows, cols], scale fp32): one scale per 128
+        values of a row (block_rows=1) or per 128 x 128 block (block_rows=128, weights)."""
+        if out is None or scale is None:
+            q, s = self.empty_quantised(*x.shape, block_rows)
+            out, scale = out or q, scale or s
+        tx, tq, ts = x.c(), out.c(), scale.c()
+        self._check(_lib.hb_quantize(self._h, C.byref(tx), C.byref(tq), C.byref(ts), block_rows))
+        return out, scale
+
+    def rmsnorm_quant(self, x: Tensor, gain: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None,
+                      eps: float = 1e-5, residual: Optional[Tensor] = None):
+        """RMSNorm (after residual += x in place, if given) quantised to (q, scale)."""
+        if out is None or scale is None:
+            q, s = self.empty_quantised(*x.shape)
+            out, scale = out or q, scale or s
+        tx, tq, ts = x.c(), out.c(), scale.c()
+        tr = C.byref(residual.c()) if residual is not None else None
+        self._check(_lib.hb_rmsnorm_quant(self._h, C.byref(tx), gain.ptr, C.byref(tq), C.byref(ts), tr, eps))
+        return out, scale
+
+    def swiglu_quant(self, x: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None):
+        """silu(x[:, :half]) * x[:, half:] quantised to (q, scale)."""
+        if out is None or scale is None:
+            q, s = self.empty_quantised(x.shape[0], x.shape[1] // 2)
+            out, scale = out or q, scale or s
+        tx, tq, ts = x.c(), out.c(), scale.c()
+        self._check(_lib.hb_swiglu_quant(self._h, C.byref(tx), C.byref(tq), C.byref(ts)))
+        return out, scale
+
+    def matmul_scaled(self, A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, out: Optional[Tensor] = None,
+                      epilogue: int = HB_EPI_NONE, residual: Optional[Tensor] = None, weights: bool = False) -> Tensor:
+        """out[M,N] bf16 = epilogue(A @ B) of two quantised matrices: A [M,K] with a scale per row
+        and 128 k, B [K,N] the `.T` of a weight matrix quantised in 128 x 128 blocks and b_scale
+        the `.T` of its scales.  `weights` as for :meth:`matmul`."""
+        M, N = A.shape[0], B.shape[1]
+        if out is None:
+            out = self.empty((M, N // 2 if epilogue == HB_EPI_SWIGLU else N), HB_BF16)
+        opts = _capi.hb_matmul_opts(epilogue | (_capi.HB_MATMUL_WEIGHTS_B if weights else 0), -1,
+                                    residual.ptr if residual else None, residual.stride[0] if residual else 0)
+        ta, tas, tb, tbs, tc = A.c(), a_scale.c(), B.c(), b_scale.c(), out.c()
+        self._check(_lib.hb_matmul_scaled(self._h, C.byref(ta), C.byref(tas), C.byref(tb), C.byref(tbs), C.byref(tc),
+                                          C.byref(opts)))
         return out
 
     # -- collective node ------------------------------------------------------------

@@ -43,7 +43,9 @@ enum {
   HB_ERR_NOMEM = 8
 };
 
-enum { HB_F32 = 0, HB_BF16 = 1, HB_I32 = 2 };
+/* HB_E4M3: 8-bit floating point, 4 exponent and 3 mantissa bits, largest value 448, no infinities
+ * (hb_quantize and the operators beside it; no other operator takes it). */
+enum { HB_F32 = 0, HB_BF16 = 1, HB_I32 = 2, HB_E4M3 = 3 };
 
 /* POD tensor view: `ptr` is a DEVICE pointer, strides are in ELEMENTS. */
 typedef struct hb_tensor {
@@ -220,6 +222,43 @@ hb_status hb_adam_step_async(hb_ctx* ctx, float* w, float* m, float* v, const vo
                        int64_t step, float grad_scale);
 /* argmax over the last dimension, first index wins ties (bit-exact). */
 hb_status hb_argmax(hb_ctx* ctx, const void* x, int32_t* out, int64_t rows, int64_t cols);
+
+/* ---- 8-bit path: e4m3 operands with one fp32 scale per 128 values --------------------
+ * A quantised matrix is a pair (q, scale).  q [rows, cols] is HB_E4M3 with contiguous rows;
+ * scale is HB_F32 and holds one value per 128 consecutive values of a row (block_rows = 1:
+ * activations, scale [rows, ceil(cols/128)]) or per 128 x 128 block (block_rows = 128: weights,
+ * scale [ceil(rows/128), ceil(cols/128)]); the last block of a row or column may be short.
+ *     scale = max(max|y| / 448, 2^-126)      q = e4m3(y / scale), nearest, ties to even
+ * and the pair stands for q * scale.  A NaN in y becomes a NaN in q and leaves its neighbours
+ * alone; an infinity makes the scale infinite, so its whole block stands for NaN.  Scale tensors
+ * may have any strides that give every element its own place.  Outputs must not overlap inputs.
+ * All sums, statistics and scales are fp32.  No reference counterpart.
+ *
+ *   hb_quantize        y = x, bf16 or fp32, [rows, cols] with contiguous rows.
+ *   hb_rmsnorm_quant   y = x * rsqrt(mean(x^2) + eps) * gain.  With `residual_inout` (may be
+ *                      NULL) residual += x first, in place and rounded to bf16, and the norm is
+ *                      taken of the updated residual, as in hb_rmsnorm.  y is not rounded to bf16
+ *                      on the way.  x, residual: bf16, cols a multiple of 8, at most 16384, rows
+ *                      16-byte aligned; q rows 8-byte aligned.
+ *   hb_swiglu_quant    y = silu(x[:, :half]) * x[:, half:] for x bf16 [rows, 2 * half]; half a
+ *                      multiple of 8, x rows 16-byte and q rows 8-byte aligned.
+ *   hb_matmul_scaled   C[M,N] = epilogue(A . B), C bf16 row-major, A [M,K] a row-quantised matrix
+ *                      (a_scale [M, ceil(K/128)]), B [K,N] the transposed view of a
+ *                      block-quantised weight matrix [N,K] (K contiguous; b_scale
+ *                      [ceil(K/128), ceil(N/128)], the transposed view of its scales).  Products
+ *                      of 128 consecutive k are summed on the tensor cores, scaled by
+ *                      a_scale * b_scale and added in fp32; C is rounded once.  A and B need
+ *                      16-byte aligned bases and row pitches that are multiples of 16; M, N and K
+ *                      are free.  `opts` as for hb_matmul (epilogues and HB_MATMUL_WEIGHTS_B;
+ *                      config_id must be -1); a residual must not overlap C.
+ * The product of few rows keeps fp32 partial sums in context scratch of a fixed size: calls of
+ * one context on different streams must be ordered by the caller, as for hb_matmul. */
+hb_status hb_quantize(hb_ctx* ctx, const hb_tensor* x, hb_tensor* q, hb_tensor* scale, int32_t block_rows);
+hb_status hb_rmsnorm_quant(hb_ctx* ctx, const hb_tensor* x, const void* gain, hb_tensor* q, hb_tensor* scale,
+                           hb_tensor* residual_inout, float eps);
+hb_status hb_swiglu_quant(hb_ctx* ctx, const hb_tensor* x, hb_tensor* q, hb_tensor* scale);
+hb_status hb_matmul_scaled(hb_ctx* ctx, const hb_tensor* A, const hb_tensor* a_scale, const hb_tensor* B,
+                           const hb_tensor* b_scale, hb_tensor* C, const hb_matmul_opts* opts);
 
 /* ---- model-IR collective node ----------------------------------------------------
  * Sum-allreduce of `count` bf16/f32 elements in place across the ranks of the
