@@ -2,9 +2,18 @@
 //
 //   C[m, n] = epilogue( sum over k-blocks of 128:  a_scale[m, kb] * b_scale[n / 128, kb] * sum_k A[m, k] B[n, k] )
 //
-// This is the plain kernel: a 64 x 64 tile per CTA, operands widened to fp32 in shared memory, the
-// sum of one k-block kept apart from the running sum so that the scales are applied once per block.
-#include <cuda_fp8.h>
+// The tensor cores sum one k-block (four tcgen05.mma of K = 32) into a slot of tensor memory; the
+// scales differ from block to block, so the running sum cannot stay there.  Eight warps take each
+// finished slot into registers and add it, times a_scale * b_scale, to fp32 accumulators that they
+// hold for the whole tile: one packed multiply-add per two outputs and k-block.  One tensor-memory
+// lane is one row of the tile and a warp's columns lie inside one 128-wide block of B, so the
+// factor is one register per thread and k-block.  The slots (two of 256 columns, or four) let the
+// tensor cores work on the next k-blocks meanwhile.
+//
+// Warp roles as in the bf16 product: warp 0 loads (TMA, 128-byte rows of one k-block, 128-byte
+// swizzle), warp 1 issues the MMAs, warps 2..9 take the sums and write the tile.
+// Algorithmic traffic per launch: M*K + N*K + 2*M*N bytes and the scales; work 2*M*N*K flop at the
+// 8-bit tensor rate (twice that of bf16).
 #include <string.h>
 
 #include <new>
@@ -14,7 +23,12 @@
 
 namespace {
 
-constexpr int KB = 128;          // k per scale
+using namespace hb;
+
+constexpr int KB = 128;          // k per scale, and bytes of a row that one ring stage holds
+constexpr int UMMA_K = 32;
+constexpr int TILE_THREADS = 320;
+constexpr int EPI_WARPS = 8;
 
 struct ScaledArgs {
   const uint8_t* A;              // [M, lda]
@@ -28,63 +42,461 @@ struct ScaledArgs {
   int b_is_weights;
 };
 
+struct TileParams {
+  const float* sa;
+  const float* sb;
+  __nv_bfloat16* C;
+  const __nv_bfloat16* R;
+  int64_t ldc, ldr, sa_m, sa_k, sb_n, sb_k;
+  int M, N, num_kb, nblocks;     // nblocks: 128-wide blocks of B
+  int tiles_m, tiles_n, raster_group;
+  int epilogue;
+  int tma_store;
+  int32_t* status;
+};
+
+// Output staging: each epilogue warp owns two buffers of 32 rows x 32 bf16 columns (64-byte rows,
+// 64-byte swizzle: the 16-byte piece c of row r sits at piece c ^ ((r >> 1) & 3)).
+constexpr int STAGE_BUF_BYTES = 32 * 64;
+constexpr int STAGE_BYTES = EPI_WARPS * 2 * STAGE_BUF_BYTES;
+
+template <bool PAIR, int BN, int STAGES>
+struct TileLayout {
+  static constexpr int BM = PAIR ? 256 : 128;
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;      // rows of B that one CTA loads
+  static constexpr int A_BYTES = 128 * KB;
+  static constexpr int B_BYTES = B_ROWS * KB;
+  static constexpr int SLOTS = BN == 256 ? 2 : 4;
+  static constexpr uint32_t TMEM_COLS = SLOTS * BN;      // 512, 512 or 256: a power of two
+  static constexpr int OFF_A = 0;
+  static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
+  static constexpr int OFF_STAGE = OFF_B + STAGES * B_BYTES;
+  static constexpr int OFF_BAR = OFF_STAGE + STAGE_BYTES;
+  static constexpr int NUM_BARS = 2 * STAGES + 2 * SLOTS;   // full, empty, tfull, tempty
+  static constexpr int OFF_TMEM_PTR = OFF_BAR + NUM_BARS * 8;
+  static constexpr int OFF_ABORT = OFF_TMEM_PTR + 4;
+  static constexpr int TOTAL = OFF_ABORT + 4;
+  static constexpr int DYN_BYTES = TOTAL + 1024;         // slack for 1024-byte alignment
+  static_assert(DYN_BYTES <= 227 * 1024, "ring does not fit shared memory");
+};
+
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
 __device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
 
-__device__ __forceinline__ float from_e4m3(uint8_t v) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
+// kind::f8f6f4, both operands e4m3 (format 0) and K-major, fp32 sums:
+//   [4,6) D format (1 = f32)   [17,23) N >> 3   [24,29) M >> 4
+constexpr uint32_t umma_idesc_e4m3(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+template <int CTA_GROUP>
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CTA_GROUP == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 
-constexpr int T = 64, TK = 32;
+// Waits for this thread's tensor-memory loads.  The registers go through the statement, so that no
+// use of them can be moved in front of it.
+__device__ __forceinline__ void tmem_wait_ld_into(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :: "memory");
+}
+// Two sums at once: acc += t * f.
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t t0, uint32_t t1, uint64_t f) {
+  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(t0), "r"(t1), "l"(f));
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
 
-__global__ void __launch_bounds__(256) hb_matmul_scaled_plain_kernel(const ScaledArgs p) {
-  __shared__ float a[TK][T + 1], b[TK][T + 1];
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * T, n0 = static_cast<int64_t>(blockIdx.x) * T;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;       // 4 x 4 outputs: rows ty * 4 + i, columns tx * 4 + j
-  float acc[4][4] = {};
-  for (int64_t kb = 0; kb * KB < p.K; ++kb) {
-    float part[4][4] = {};
-    for (int k0 = 0; k0 < KB; k0 += TK) {
-      for (int i = threadIdx.x; i < T * TK; i += 256) {
-        const int r = i / TK, kk = i % TK;
-        const int64_t k = kb * KB + k0 + kk;
-        a[kk][r] = m0 + r < p.M && k < p.K ? from_e4m3(p.A[(m0 + r) * p.lda + k]) : 0.f;
-        b[kk][r] = n0 + r < p.N && k < p.K ? from_e4m3(p.B[(n0 + r) * p.ldb + k]) : 0.f;
-      }
-      __syncthreads();
-      for (int kk = 0; kk < TK; ++kk)
+__device__ __forceinline__ void tile_coords(int tile, const TileParams& p, int& tm, int& tn) {
+  // N is swept inside groups of M-tiles, so that CTAs that run together share rows of A and B in L2
+  const int per_group = p.raster_group * p.tiles_n;
+  const int group = tile / per_group;
+  const int first_m = group * p.raster_group;
+  const int rows = min(p.raster_group, p.tiles_m - first_m);
+  const int in_group = tile - group * per_group;
+  tm = first_m + in_group % rows;
+  tn = in_group / rows;
+}
+
+// 32 output columns of one row from col0 on, in fp32, rounded once and stored: through the warp's
+// staging buffer and TMA (whole lines, clipped at the matrix edge), or straight to memory where C's
+// base or pitch allow no tensor map.  `chunk` counts the warp's staged blocks over all tiles.
+__device__ __forceinline__ void store_chunk(const TileParams& p, const CUtensorMap* tmC, uint32_t stage, int lane, int row0,
+                                            int col0, int ncols, int& chunk, const float (&f)[32]) {
+  uint32_t o[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+  for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+  if (p.tma_store) {
+    stage += (chunk & 1) * STAGE_BUF_BYTES;
+    ++chunk;
+    if (lane == 0) tma_store_wait_read<1>();     // the store issued two blocks ago has read this buffer
+    __syncwarp();
+    const uint32_t mine = stage + lane * 64;
+    const int sw = (lane >> 1) & 3;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] += a[kk][ty * 4 + i] * b[kk][tx * 4 + j];
-      __syncthreads();
+    for (int c = 0; c < 4; ++c)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ sw) << 4)), "r"(o[4 * c]), "r"(o[4 * c + 1]),
+                   "r"(o[4 * c + 2]), "r"(o[4 * c + 3])
+                   : "memory");
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (row0 < p.M && col0 < ncols) tma_store_2d(tmC, stage, col0, row0);
+      tma_store_commit();
     }
+  } else if (row0 + lane < p.M) {
+    __nv_bfloat16* dst = p.C + static_cast<int64_t>(row0 + lane) * p.ldc + col0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < ncols) dst[j] = __ushort_as_bfloat16(static_cast<unsigned short>(o[j >> 1] >> 16 * (j & 1)));
+  }
+}
+
+// The accumulators of one thread (row `row0 + lane`, HALF columns from col0 on) -> C.
+template <int HALF>
+__device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMap* tmC, uint32_t stage, int lane, int row0,
+                                           int col0, int& chunk, const uint64_t (&acc)[HALF / 2]) {
+  if (HALF >= 64 && p.epilogue == HB_EPI_SWIGLU) {
+    // columns interleave (gate, up): 64 sums give 32 outputs
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-        if (m < p.M && n < p.N) acc[i][j] += part[i][j] * (p.sa[m * p.sa_m + kb * p.sa_k] * p.sb[n / KB * p.sb_n + kb * p.sb_k]);
+    for (int c = 0; c < HALF / 64; ++c) {
+      float f[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float2 gu = unpack2(acc[c * 32 + j]);
+        f[j] = silu(gu.x) * gu.y;
       }
+      store_chunk(p, tmC, stage, lane, row0, (col0 >> 1) + c * 32, p.N >> 1, chunk, f);
+    }
+    return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty * 4 + i;
-    if (m >= p.M) continue;
+  for (int c = 0; c < HALF / 32; ++c) {
+    float f[32];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t n = n0 + tx * 4 + j;
-      if (n >= p.N) continue;
-      if (p.epilogue == HB_EPI_SWIGLU) {
-        if (!(j & 1)) p.C[m * p.ldc + n / 2] = __float2bfloat16_rn(silu(acc[i][j]) * acc[i][j + 1]);
-        continue;
-      }
-      float v = acc[i][j];
-      if (p.epilogue == HB_EPI_GELU) v = gelu_erf(v);
-      if (p.epilogue == HB_EPI_RESIDUAL) v += __bfloat162float(p.R[m * p.ldr + n]);
-      p.C[m * p.ldc + n] = __float2bfloat16_rn(v);
+    for (int j = 0; j < 16; ++j) {
+      const float2 v = unpack2(acc[c * 16 + j]);
+      f[2 * j] = v.x;
+      f[2 * j + 1] = v.y;
     }
+    const int col = col0 + c * 32;
+    if (p.epilogue == HB_EPI_GELU) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
+    } else if (p.epilogue == HB_EPI_RESIDUAL && row0 + lane < p.M) {
+      const __nv_bfloat16* r = p.R + static_cast<int64_t>(row0 + lane) * p.ldr + col;
+      if ((p.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(p.R) & 15) == 0 && col + 32 <= p.N) {
+#pragma unroll
+        for (int j4 = 0; j4 < 4; ++j4) {
+          const uint4 rv = *(reinterpret_cast<const uint4*>(r) + j4);
+          const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f[j4 * 8 + 2 * j] += __uint_as_float(rw[j] << 16);
+            f[j4 * 8 + 2 * j + 1] += __uint_as_float(rw[j] & 0xffff0000u);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (col + j < p.N) f[j] += __bfloat162float(r[j]);
+      }
+    }
+    store_chunk(p, tmC, stage, lane, row0, col, p.N, chunk, f);
   }
+}
+
+__device__ __forceinline__ void report_timeout(int32_t* status, int what) {
+  if (status) { atomicCAS(status, 0, HB_ERR_TIMEOUT); status[1] = HB_KTAG_SCALED; status[2] = what; }
+}
+
+template <bool PAIR, int BN, int STAGES>
+__device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC,
+                                                 const TileParams& p) {
+  using L = TileLayout<PAIR, BN, STAGES>;
+  constexpr int GROUP = PAIR ? 2 : 1;
+  constexpr int HALF = BN / 2;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t sA = smem_base + L::OFF_A;
+  const uint32_t sB = smem_base + L::OFF_B;
+  const uint32_t bar_full = smem_base + L::OFF_BAR;
+  const uint32_t bar_empty = bar_full + STAGES * 8;
+  const uint32_t bar_tfull = bar_empty + STAGES * 8;
+  const uint32_t bar_tempty = bar_tfull + L::SLOTS * 8;
+  volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_TMEM_PTR);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_ABORT);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = blockIdx.x / GROUP;               // CTA or pair
+  const int num_units = gridDim.x / GROUP;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(bar_full + s * 8, GROUP);
+      mbar_init(bar_empty + s * 8, 1);
+    }
+    for (int a = 0; a < L::SLOTS; ++a) {
+      mbar_init(bar_tfull + a * 8, 1);
+      mbar_init(bar_tempty + a * 8, EPI_WARPS * GROUP);
+    }
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc<GROUP>(smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)), L::TMEM_COLS);
+    tmem_relinquish<GROUP>();
+  }
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync(); else __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  const int num_tiles = p.tiles_m * p.tiles_n;
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
+        int tm, tn;
+        tile_coords(tile, p, tm, tn);
+        const int m0 = tm * L::BM + rank * 128, n0 = tn * BN + rank * L::B_ROWS;
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
+          if constexpr (PAIR) {
+            const uint32_t full_leader = mapa(bar_full + s * 8, 0);
+            if (rank == 0) mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
+            else mbar_arrive_expect_tx_cluster(full_leader, L::A_BYTES + L::B_BYTES);
+            tma_load_2d_pair(sA + s * L::A_BYTES, &tmA, full_leader, kb * KB, m0);
+            tma_load_2d_pair(sB + s * L::B_BYTES, &tmB, full_leader, kb * KB, n0);
+          } else {
+            mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
+            tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, kb * KB, m0);
+            tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, kb * KB, n0);
+          }
+          if (++s == STAGES) { s = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) report_timeout(p.status, 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (of a pair: the leader)
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_e4m3(L::BM, BN);
+      int s = 0, slot = 0;
+      uint32_t phase = 0, slot_phase = 0;
+      bool ok = true;
+      for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!mbar_wait(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag) || !mbar_wait(bar_full + s * 8, phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < KB / UMMA_K; ++k)
+            umma_e4m3<GROUP>(tmem_base + slot * BN, umma_desc_k_sw128(sA + s * L::A_BYTES + k * UMMA_K),
+                             umma_desc_k_sw128(sB + s * L::B_BYTES + k * UMMA_K), idesc, k != 0 ? 1u : 0u);
+          if constexpr (PAIR) {
+            umma_commit_pair_mcast(bar_empty + s * 8, 3);
+            umma_commit_pair_mcast(bar_tfull + slot * 8, 3);
+          } else {
+            umma_commit<1>(bar_empty + s * 8);
+            umma_commit<1>(bar_tfull + slot * 8);
+          }
+          if (++s == STAGES) { s = 0; phase ^= 1; }
+          if (++slot == L::SLOTS) { slot = 0; slot_phase ^= 1; }
+        }
+      }
+      if (!ok) report_timeout(p.status, 2);
+    }
+  } else {
+    // ------------------------------------------------------------ sums (warps 2..9)
+    const int q = warp & 3;                          // tensor-memory lanes this warp may read
+    const int h = (warp - 2) >> 2;                   // half of the tile's columns
+    const uint32_t stage_mine = smem_base + L::OFF_STAGE + (warp - 2) * 2 * STAGE_BUF_BYTES;
+    const uint32_t t_mine = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * HALF;
+    uint32_t tempty = bar_tempty;
+    if constexpr (PAIR) tempty = mapa(bar_tempty, 0);
+    int slot = 0, chunk = 0;
+    uint32_t slot_phase = 0;
+    bool ok = true;
+    for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
+      int tm, tn;
+      tile_coords(tile, p, tm, tn);
+      const int row0 = tm * L::BM + rank * 128 + q * 32;
+      const int col0 = tn * BN + h * HALF;
+      // rows and blocks past the edge repeat the last one: their sums are zero and are not stored
+      const float* sa = p.sa + min(row0 + lane, p.M - 1) * p.sa_m;
+      const float* sb = p.sb + min(col0 / KB, p.nblocks - 1) * p.sb_n;
+      uint64_t acc[HALF / 2];
+#pragma unroll
+      for (int j = 0; j < HALF / 2; ++j) acc[j] = 0;
+      float fa = __ldg(sa), fb = __ldg(sb);
+      for (int kb = 0; kb < p.num_kb; ++kb) {
+        const uint64_t f = pack2(fa * fb, fa * fb);
+        if (kb + 1 < p.num_kb) {                     // the next block's scales arrive under this block's sums
+          fa = __ldg(sa + (kb + 1) * p.sa_k);
+          fb = __ldg(sb + (kb + 1) * p.sb_k);
+        }
+        if (!mbar_wait(bar_tfull + slot * 8, slot_phase, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t t = t_mine + slot * BN;
+        uint32_t v[2][16];
+        tmem_ld_32x16(t, v[0]);
+#pragma unroll
+        for (int c = 0; c < HALF / 16; ++c) {
+          tmem_wait_ld_into(v[c & 1]);
+          if (c + 1 < HALF / 16) {
+            tmem_ld_32x16(t + (c + 1) * 16, v[(c + 1) & 1]);
+          } else {                                   // everything is in registers: the slot is free
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR) mbar_arrive_cluster(tempty + slot * 8);
+              else mbar_arrive(tempty + slot * 8);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
+        }
+        if (++slot == L::SLOTS) { slot = 0; slot_phase ^= 1; }
+      }
+      if (ok) write_half<HALF>(p, &tmC, stage_mine, lane, row0, col0, chunk, acc);
+    }
+    if (p.tma_store && lane == 0) tma_store_wait<0>();   // the staged blocks have left shared memory and landed
+    if (!ok && lane == 0) report_timeout(p.status, 3);
+  }
+
+  // ---------------------------------------------------------------- teardown
+  // of a pair, neither CTA may leave while its partner can still signal its barriers or read its
+  // shared memory
+  tc_fence_before();
+  if constexpr (PAIR) cluster_sync(); else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<GROUP>(tmem_base, L::TMEM_COLS);
+  }
+}
+
+template <int BN, int STAGES>
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+hb_matmul_scaled_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                        const __grid_constant__ CUtensorMap tmC, const __grid_constant__ TileParams p) {
+  scaled_tile_body<false, BN, STAGES>(tmA, tmB, tmC, p);
+}
+template <int BN, int STAGES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
+hb_matmul_scaled_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                             const __grid_constant__ CUtensorMap tmC, const __grid_constant__ TileParams p) {
+  scaled_tile_body<true, BN, STAGES>(tmA, tmB, tmC, p);
+}
+
+hb_status make_maps(hb_ctx* ctx, const ScaledArgs& g, int b_rows, CUtensorMap* tmA, CUtensorMap* tmB, CUtensorMap* tmC, int* tma_store) {
+  uint64_t dims[2] = {(uint64_t)g.K, (uint64_t)g.M}, pitch[1] = {(uint64_t)g.lda};
+  uint32_t box[2] = {KB, 128};
+  hb_status st = hb_make_tensor_map(ctx, tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, g.A, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != HB_OK) return st;
+  dims[1] = (uint64_t)g.N; pitch[0] = (uint64_t)g.ldb; box[1] = (uint32_t)b_rows;
+  if ((st = hb_make_tensor_map(ctx, tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, g.B, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B)) != HB_OK) return st;
+  *tmC = *tmA;
+  const bool one_row = g.M == 1;                 // its pitch is never used
+  const int64_t cols = g.epilogue == HB_EPI_SWIGLU ? g.N / 2 : g.N;
+  // TMA clips a store at whole 16-byte pieces: a row that ends inside one would be written to the
+  // piece's end (measured: a single-column store put seven zeros behind it)
+  *tma_store = (cols & 7) == 0 && (one_row || (g.ldc & 7) == 0) && (reinterpret_cast<uintptr_t>(g.C) & 15) == 0;
+  if (*tma_store) {
+    dims[0] = (uint64_t)cols; dims[1] = (uint64_t)g.M; pitch[0] = (uint64_t)(one_row ? cols : g.ldc) * 2;
+    box[0] = 32; box[1] = 32;
+    st = hb_make_tensor_map(ctx, tmC, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.C, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  return st;
+}
+
+template <bool PAIR, int BN, int STAGES>
+hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g) {
+  using L = TileLayout<PAIR, BN, STAGES>;
+  void (*kern)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const TileParams);
+  if constexpr (PAIR) kern = hb_matmul_scaled_pair_kernel<BN, STAGES>;
+  else kern = hb_matmul_scaled_kernel<BN, STAGES>;
+  // persistent CTAs (or pairs) that can run at once; of pairs the occupancy query knows, because not
+  // every SM has a neighbour to pair with
+  static int resident[64] = {};
+  if (!resident[ctx->device & 63]) {
+    HB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN_BYTES));
+    int n = ctx->sm_count;
+    if constexpr (PAIR) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(ctx->sm_count & ~1u);
+      cfg.blockDim = dim3(TILE_THREADS);
+      cfg.dynamicSmemBytes = L::DYN_BYTES;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) { cudaGetLastError(); n = ctx->sm_count / 2 - 8; }
+    }
+    resident[ctx->device & 63] = n;
+  }
+  CUtensorMap tmA, tmB, tmC;
+  TileParams p;
+  memset(&p, 0, sizeof(p));
+  const hb_status st = make_maps(ctx, g, L::B_ROWS, &tmA, &tmB, &tmC, &p.tma_store);
+  if (st != HB_OK) return st;
+  p.sa = g.sa; p.sb = g.sb; p.C = g.C; p.R = g.R;
+  p.ldc = g.ldc; p.ldr = g.ldr;
+  p.sa_m = g.sa_m; p.sa_k = g.sa_k; p.sb_n = g.sb_n; p.sb_k = g.sb_k;
+  p.M = (int)g.M; p.N = (int)g.N;
+  p.num_kb = (int)((g.K + KB - 1) / KB);
+  p.nblocks = (int)((g.N + KB - 1) / KB);
+  const int64_t tiles_m = (g.M + L::BM - 1) / L::BM, tiles_n = (g.N + BN - 1) / BN;
+  if (tiles_m * tiles_n > INT32_MAX / 2) return hb_fail(ctx, HB_ERR_UNSUPPORTED, "matmul_scaled: problem too large");
+  p.tiles_m = (int)tiles_m; p.tiles_n = (int)tiles_n;
+  p.raster_group = 8;
+  p.epilogue = g.epilogue;
+  p.status = ctx->d_status;
+  const int tiles = p.tiles_m * p.tiles_n, most = resident[ctx->device & 63];
+  const unsigned ctas = (PAIR ? 2 : 1) * (unsigned)(tiles < most ? tiles : most);
+  const cudaError_t e = hb_launch_dependent(kern, dim3(ctas), dim3(TILE_THREADS), L::DYN_BYTES, ctx->stream, tmA, tmB, tmC, p);
+  if (e != cudaSuccess) { cudaGetLastError(); return hb_check_cuda(ctx, e, "matmul_scaled launch"); }
+  ctx->launches++;
+  return HB_OK;
+}
+
+hb_status launch(hb_ctx* ctx, const ScaledArgs& g) {
+  if (g.M > 128 && g.N > 128) return launch_tile<true, 256, 6>(ctx, g);
+  return launch_tile<false, 128, 5>(ctx, g);
 }
 
 hb_status decode(hb_ctx* ctx, const hb_tensor* A, const hb_tensor* sa, const hb_tensor* B, const hb_tensor* sb,
@@ -149,11 +561,7 @@ hb_status matmul_scaled(hb_ctx* ctx, const hb_tensor* A, const hb_tensor* sa, co
   const hb_status st = decode(ctx, A, sa, B, sb, C, opts, &g);
   if (st != HB_OK) return st;
   hb_device_guard guard(ctx);
-  const dim3 grid((unsigned)((g.N + T - 1) / T), (unsigned)((g.M + T - 1) / T));
-  if (grid.y > 65535) return hb_fail(ctx, HB_ERR_UNSUPPORTED, "matmul_scaled: too many rows");
-  hb_matmul_scaled_plain_kernel<<<grid, 256, 0, ctx->stream>>>(g);
-  ctx->launches++;
-  return hb_check_cuda(ctx, cudaGetLastError(), "matmul_scaled launch");
+  return launch(ctx, g);
 }
 
 }  // namespace
