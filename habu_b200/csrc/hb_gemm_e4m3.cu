@@ -10,8 +10,10 @@
 // factor is one register per thread and k-block.  The slots (two of 256 columns, or four) let the
 // tensor cores work on the next k-blocks meanwhile.
 //
-// Warp roles as in the bf16 product: warp 0 loads (TMA, 128-byte rows of one k-block, 128-byte
-// swizzle), warp 1 issues the MMAs, warps 2..9 take the sums and write the tile.
+// Warp roles: warp 0 loads (TMA, 128-byte rows of one k-block, 128-byte swizzle), warp 1 issues the
+// MMAs, warps 4..11 take the sums and write the tile.  The accumulators need more registers than
+// an even share, so the first four warps hand some of theirs over (setmaxnreg; the shares add up to
+// what the launch holds).
 // Algorithmic traffic per launch: M*K + N*K + 2*M*N bytes and the scales; work 2*M*N*K flop at the
 // 8-bit tensor rate (twice that of bf16).
 #include <string.h>
@@ -27,8 +29,10 @@ using namespace hb;
 
 constexpr int KB = 128;          // k per scale, and bytes of a row that one ring stage holds
 constexpr int UMMA_K = 32;
-constexpr int TILE_THREADS = 320;
-constexpr int EPI_WARPS = 8;
+constexpr int TILE_THREADS = 384;
+constexpr int EPI_WARP0 = 4, EPI_WARPS = 8;
+constexpr int REGS_LAUNCH = 168, REGS_FEW = 40, REGS_MANY = 232;   // per thread, multiples of 8
+static_assert(REGS_FEW + 2 * REGS_MANY <= 3 * REGS_LAUNCH && TILE_THREADS * REGS_LAUNCH <= 65536, "register split");
 
 struct ScaledArgs {
   const uint8_t* A;              // [M, lda]
@@ -55,10 +59,12 @@ struct TileParams {
   int32_t* status;
 };
 
-// Output staging: each epilogue warp owns two buffers of 32 rows x 32 bf16 columns (64-byte rows,
-// 64-byte swizzle: the 16-byte piece c of row r sits at piece c ^ ((r >> 1) & 3)).
+// Output staging: each epilogue warp owns four buffers of 32 rows x 32 bf16 columns (64-byte rows,
+// 64-byte swizzle: the 16-byte piece c of row r sits at piece c ^ ((r >> 1) & 3)), enough for its
+// share of a tile, so that one proxy fence covers all of a tile's stores.
 constexpr int STAGE_BUF_BYTES = 32 * 64;
-constexpr int STAGE_BYTES = EPI_WARPS * 2 * STAGE_BUF_BYTES;
+constexpr int STAGE_BUFS = 4;
+constexpr int STAGE_BYTES = EPI_WARPS * STAGE_BUFS * STAGE_BUF_BYTES;
 
 template <bool PAIR, int BN, int STAGES>
 struct TileLayout {
@@ -81,7 +87,8 @@ struct TileLayout {
 };
 
 __device__ __forceinline__ float gelu_erf(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f)); }
-__device__ __forceinline__ float silu(float x) { return x / (1.0f + __expf(-x)); }
+// approximate exponential and division, 2 ulp each; far below zero the denominator is infinite and the quotient -0
+__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
 
 // kind::f8f6f4, both operands e4m3 (format 0) and K-major, fp32 sums:
 //   [4,6) D format (1 = f32)   [17,23) N >> 3   [24,29) M >> 4
@@ -104,17 +111,9 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
 }
 
-// Waits for this thread's tensor-memory loads.  The registers go through the statement, so that no
-// use of them can be moved in front of it.
-__device__ __forceinline__ void tmem_wait_ld_into(uint32_t (&v)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
-                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
-               :: "memory");
-}
-// Two sums at once: acc += t * f.
+// Two sums at once: acc += t * f.  Volatile like the tensor-memory load and the wait for it, so that it stays behind both.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t t0, uint32_t t1, uint64_t f) {
-  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(t0), "r"(t1), "l"(f));
+  asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(t0), "r"(t1), "l"(f));
 }
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
   uint64_t v;
@@ -138,32 +137,22 @@ __device__ __forceinline__ void tile_coords(int tile, const TileParams& p, int& 
   tn = in_group / rows;
 }
 
-// 32 output columns of one row from col0 on, in fp32, rounded once and stored: through the warp's
-// staging buffer and TMA (whole lines, clipped at the matrix edge), or straight to memory where C's
-// base or pitch allow no tensor map.  `chunk` counts the warp's staged blocks over all tiles.
-__device__ __forceinline__ void store_chunk(const TileParams& p, const CUtensorMap* tmC, uint32_t stage, int lane, int row0,
-                                            int col0, int ncols, int& chunk, const float (&f)[32]) {
+// 32 output columns of one row from col0 on, rounded once: into staging buffer `buf` of the warp (the
+// caller hands it to TMA, which writes whole lines and clips the block at the matrix edge), or
+// straight to memory where C's base, pitch or width allow no tensor map.
+__device__ __forceinline__ void put_chunk(const TileParams& p, uint32_t stage, int buf, int lane, int row0, int col0, int ncols,
+                                          const float (&f)[32]) {
   uint32_t o[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
   if (p.tma_store) {
-    stage += (chunk & 1) * STAGE_BUF_BYTES;
-    ++chunk;
-    if (lane == 0) tma_store_wait_read<1>();     // the store issued two blocks ago has read this buffer
-    __syncwarp();
-    const uint32_t mine = stage + lane * 64;
+    const uint32_t mine = stage + buf * STAGE_BUF_BYTES + lane * 64;
     const int sw = (lane >> 1) & 3;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ sw) << 4)), "r"(o[4 * c]), "r"(o[4 * c + 1]),
                    "r"(o[4 * c + 2]), "r"(o[4 * c + 3])
                    : "memory");
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (row0 < p.M && col0 < ncols) tma_store_2d(tmC, stage, col0, row0);
-      tma_store_commit();
-    }
   } else if (row0 + lane < p.M) {
     __nv_bfloat16* dst = p.C + static_cast<int64_t>(row0 + lane) * p.ldc + col0;
 #pragma unroll
@@ -175,8 +164,13 @@ __device__ __forceinline__ void store_chunk(const TileParams& p, const CUtensorM
 // The accumulators of one thread (row `row0 + lane`, HALF columns from col0 on) -> C.
 template <int HALF>
 __device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMap* tmC, uint32_t stage, int lane, int row0,
-                                           int col0, int& chunk, const uint64_t (&acc)[HALF / 2]) {
-  if (HALF >= 64 && p.epilogue == HB_EPI_SWIGLU) {
+                                           int col0, const uint64_t (&acc)[HALF / 2]) {
+  if (p.tma_store) {
+    if (lane == 0) tma_store_wait_read<0>();     // the last tile's stores have read the buffers
+    __syncwarp();
+  }
+  const bool swiglu = HALF >= 64 && p.epilogue == HB_EPI_SWIGLU;
+  if (swiglu) {
     // columns interleave (gate, up): 64 sums give 32 outputs
 #pragma unroll
     for (int c = 0; c < HALF / 64; ++c) {
@@ -186,43 +180,54 @@ __device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMa
         const float2 gu = unpack2(acc[c * 32 + j]);
         f[j] = silu(gu.x) * gu.y;
       }
-      store_chunk(p, tmC, stage, lane, row0, (col0 >> 1) + c * 32, p.N >> 1, chunk, f);
+      put_chunk(p, stage, c, lane, row0, (col0 >> 1) + c * 32, p.N >> 1, f);
     }
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int c = 0; c < HALF / 32; ++c) {
-    float f[32];
+    for (int c = 0; c < HALF / 32; ++c) {
+      float f[32];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float2 v = unpack2(acc[c * 16 + j]);
-      f[2 * j] = v.x;
-      f[2 * j + 1] = v.y;
-    }
-    const int col = col0 + c * 32;
-    if (p.epilogue == HB_EPI_GELU) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
-    } else if (p.epilogue == HB_EPI_RESIDUAL && row0 + lane < p.M) {
-      const __nv_bfloat16* r = p.R + static_cast<int64_t>(row0 + lane) * p.ldr + col;
-      if ((p.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(p.R) & 15) == 0 && col + 32 <= p.N) {
-#pragma unroll
-        for (int j4 = 0; j4 < 4; ++j4) {
-          const uint4 rv = *(reinterpret_cast<const uint4*>(r) + j4);
-          const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            f[j4 * 8 + 2 * j] += __uint_as_float(rw[j] << 16);
-            f[j4 * 8 + 2 * j + 1] += __uint_as_float(rw[j] & 0xffff0000u);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col + j < p.N) f[j] += __bfloat162float(r[j]);
+      for (int j = 0; j < 16; ++j) {
+        const float2 v = unpack2(acc[c * 16 + j]);
+        f[2 * j] = v.x;
+        f[2 * j + 1] = v.y;
       }
+      const int col = col0 + c * 32;
+      if (p.epilogue == HB_EPI_GELU) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
+      } else if (p.epilogue == HB_EPI_RESIDUAL && row0 + lane < p.M) {
+        const __nv_bfloat16* r = p.R + static_cast<int64_t>(row0 + lane) * p.ldr + col;
+        if ((p.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(p.R) & 15) == 0 && col + 32 <= p.N) {
+#pragma unroll
+          for (int j4 = 0; j4 < 4; ++j4) {
+            const uint4 rv = *(reinterpret_cast<const uint4*>(r) + j4);
+            const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f[j4 * 8 + 2 * j] += __uint_as_float(rw[j] << 16);
+              f[j4 * 8 + 2 * j + 1] += __uint_as_float(rw[j] & 0xffff0000u);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col + j < p.N) f[j] += __bfloat162float(r[j]);
+        }
+      }
+      put_chunk(p, stage, c, lane, row0, col, p.N, f);
     }
-    store_chunk(p, tmC, stage, lane, row0, col, p.N, chunk, f);
+  }
+  if (p.tma_store) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && row0 < p.M) {
+      const int first = swiglu ? col0 >> 1 : col0, ncols = swiglu ? p.N >> 1 : p.N;
+      const int n = swiglu ? HALF / 64 : HALF / 32;
+      for (int c = 0; c < n; ++c)
+        if (first + c * 32 < ncols) tma_store_2d(tmC, stage + c * STAGE_BUF_BYTES, first + c * 32, row0);
+      tma_store_commit();
+    }
   }
 }
 
@@ -281,6 +286,8 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
   grid_launch_dependents();
 
   const int num_tiles = p.tiles_m * p.tiles_n;
+  if (warp < EPI_WARP0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (elect_one()) {
@@ -318,7 +325,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       bool ok = true;
       for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag) || !mbar_wait(bar_full + s * 8, phase, abort_flag)) {
+          if (!mbar_wait_spin(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag) || !mbar_wait_spin(bar_full + s * 8, phase, abort_flag)) {
             ok = false;
             break;
           }
@@ -340,29 +347,36 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       }
       if (!ok) report_timeout(p.status, 2);
     }
+  }
   } else {
-    // ------------------------------------------------------------ sums (warps 2..9)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
+    // ------------------------------------------------------------ sums (warps 4..11)
     const int q = warp & 3;                          // tensor-memory lanes this warp may read
-    const int h = (warp - 2) >> 2;                   // half of the tile's columns
-    const uint32_t stage_mine = smem_base + L::OFF_STAGE + (warp - 2) * 2 * STAGE_BUF_BYTES;
+    const int h = (warp - EPI_WARP0) >> 2;                   // half of the tile's columns
+    const uint32_t stage_mine = smem_base + L::OFF_STAGE + (warp - EPI_WARP0) * STAGE_BUFS * STAGE_BUF_BYTES;
     const uint32_t t_mine = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + h * HALF;
     uint32_t tempty = bar_tempty;
     if constexpr (PAIR) tempty = mapa(bar_tempty, 0);
-    int slot = 0, chunk = 0;
+    int slot = 0;
     uint32_t slot_phase = 0;
     bool ok = true;
-    for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
+    // scales of this thread's row and columns in `tile`; rows and blocks past the edge repeat the last
+    // one: their sums are zero and are not stored
+    const float *sa = nullptr, *sb = nullptr;
+    float fa = 0.f, fb = 0.f;
+    auto first_scales = [&](int tile) {
       int tm, tn;
       tile_coords(tile, p, tm, tn);
-      const int row0 = tm * L::BM + rank * 128 + q * 32;
-      const int col0 = tn * BN + h * HALF;
-      // rows and blocks past the edge repeat the last one: their sums are zero and are not stored
-      const float* sa = p.sa + min(row0 + lane, p.M - 1) * p.sa_m;
-      const float* sb = p.sb + min(col0 / KB, p.nblocks - 1) * p.sb_n;
+      sa = p.sa + min(tm * L::BM + rank * 128 + q * 32 + lane, p.M - 1) * p.sa_m;
+      sb = p.sb + min((tn * BN + h * HALF) / KB, p.nblocks - 1) * p.sb_n;
+      fa = __ldg(sa);
+      fb = __ldg(sb);
+    };
+    if (unit < num_tiles) first_scales(unit);
+    for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
       uint64_t acc[HALF / 2];
 #pragma unroll
       for (int j = 0; j < HALF / 2; ++j) acc[j] = 0;
-      float fa = __ldg(sa), fb = __ldg(sb);
       for (int kb = 0; kb < p.num_kb; ++kb) {
         const uint64_t f = pack2(fa * fb, fa * fb);
         if (kb + 1 < p.num_kb) {                     // the next block's scales arrive under this block's sums
@@ -376,7 +390,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
         tmem_ld_32x16(t, v[0]);
 #pragma unroll
         for (int c = 0; c < HALF / 16; ++c) {
-          tmem_wait_ld_into(v[c & 1]);
+          tmem_wait_ld();
           if (c + 1 < HALF / 16) {
             tmem_ld_32x16(t + (c + 1) * 16, v[(c + 1) & 1]);
           } else {                                   // everything is in registers: the slot is free
@@ -392,7 +406,11 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
         }
         if (++slot == L::SLOTS) { slot = 0; slot_phase ^= 1; }
       }
-      if (ok) write_half<HALF>(p, &tmC, stage_mine, lane, row0, col0, chunk, acc);
+      int tm, tn;
+      tile_coords(tile, p, tm, tn);
+      const int row0 = tm * L::BM + rank * 128 + q * 32, col0 = tn * BN + h * HALF;
+      if (tile + num_units < num_tiles) first_scales(tile + num_units);   // arrive under this tile's output
+      if (ok) write_half<HALF>(p, &tmC, stage_mine, lane, row0, col0, acc);
     }
     if (p.tma_store && lane == 0) tma_store_wait<0>();   // the staged blocks have left shared memory and landed
     if (!ok && lane == 0) report_timeout(p.status, 3);
@@ -495,8 +513,8 @@ hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g) {
 }
 
 hb_status launch(hb_ctx* ctx, const ScaledArgs& g) {
-  if (g.M > 128 && g.N > 128) return launch_tile<true, 256, 6>(ctx, g);
-  return launch_tile<false, 128, 5>(ctx, g);
+  if (g.M > 128 && g.N > 128) return launch_tile<true, 256, 5>(ctx, g);
+  return launch_tile<false, 128, 4>(ctx, g);
 }
 
 hb_status decode(hb_ctx* ctx, const hb_tensor* A, const hb_tensor* sa, const hb_tensor* B, const hb_tensor* sb,
