@@ -512,7 +512,433 @@ hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g) {
   return HB_OK;
 }
 
+// ------------------------------------------------------------------------------------
+// Few rows (M <= 64): bound by reading B once.  The operands change places -- a slab of 128 rows of B
+// is the M side of the MMA, the rows of A, padded to 16, 32 or 64 by TMA's zero fill, its N side.
+// A cluster of S CTAs owns whole slabs and cuts their (slab, k-block) units into S contiguous ranges of
+// the same length, one per CTA, so that every SM streams the same number of bytes.  A finished k-block
+// goes to one of eight tensor-memory slots; a thread holds one column of C (one row of the slab) for
+// all rows of A, and the factors a_scale * b_scale of a k-block come through shared memory from a warp
+// that runs ahead.  Where a range starts inside a slab, its sums go to the CTA that started the slab, over
+// distributed shared memory, as the first thing that a CTA finishes; the starter comes to that slab
+// last, finds them there and adds them in k order: the same bits every run, nothing waits in
+// practice, and there is no scratch and no counter in global memory that launches could share.
+// For up to 16 rows a CTA takes less than half an SM, so that the next launch on the stream can set
+// itself up beside this one.  With HB_MATMUL_WEIGHTS_B it also fills its ring with B before the kernel
+// in front has finished (programmatic dependent launch); what depends on that kernel comes after the
+// wait.
+// ------------------------------------------------------------------------------------
+constexpr int FEW_MAX_M = 64;
+constexpr int FEW_THREADS = 224;                 // TMA, MMA, four warps of sums, factors
+constexpr int FEW_SLOTS = 8;
+constexpr int FEW_MAX_CLUSTER = 4;
+constexpr int SLAB = 128;
+
+struct FewParams {
+  const float* sa;
+  const float* sb;
+  __nv_bfloat16* C;
+  const __nv_bfloat16* R;
+  int64_t ldc, ldr, sa_m, sa_k, sb_n, sb_k;
+  int M, N, num_kb, slabs;
+  int cluster;                 // CTAs per cluster
+  int epilogue, b_is_weights;
+  int32_t* status;
+};
+
+template <int MP>
+struct FewLayout {
+  static constexpr int A_BYTES = MP * KB, B_BYTES = SLAB * KB;
+  static constexpr int CTAS_PER_SM = MP <= 16 ? 2 : 1;
+  static constexpr uint32_t TMEM_COLS = FEW_SLOTS * MP;                   // 128, 256 or 512
+  static constexpr int F_BYTES = FEW_SLOTS * MP * 4;                      // factors: [slot][MP] fp32
+  static constexpr int X_BYTES = (FEW_MAX_CLUSTER - 1) * MP * SLAB * 4;   // sums received: [sender][row of A][128] fp32
+  static constexpr int W_BYTES = 16 * SLAB * 4;                           // sixteen rows on their way out
+  static constexpr int STAGES = (227 * 1024 / CTAS_PER_SM - 4096 - F_BYTES - X_BYTES - W_BYTES) / (A_BYTES + B_BYTES);
+  static constexpr int OFF_B = 0;
+  static constexpr int OFF_A = OFF_B + STAGES * B_BYTES;
+  static constexpr int OFF_F = OFF_A + STAGES * A_BYTES;
+  static constexpr int OFF_X = OFF_F + F_BYTES;
+  static constexpr int OFF_W = OFF_X + X_BYTES;
+  static constexpr int OFF_BAR = OFF_W + W_BYTES;      // full, empty per stage; tfull, tempty, ffull per slot; xfull per warp
+  static constexpr int OFF_TMEM_PTR = OFF_BAR + (2 * STAGES + 3 * FEW_SLOTS + 4) * 8;
+  static constexpr int OFF_ABORT = OFF_TMEM_PTR + 4;
+  static constexpr int DYN_BYTES = OFF_ABORT + 4 + 1024;
+  static_assert(CTAS_PER_SM * (DYN_BYTES + 1024) <= 228 * 1024 && STAGES >= 3, "ring does not fit shared memory");
+};
+
+// Arrive on / wait for a barrier when the data it stands for crossed between CTAs of the cluster.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < HB_SPIN_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 1023u) == 1023u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+template <int MP>
+__global__ void __launch_bounds__(FEW_THREADS, FewLayout<MP>::CTAS_PER_SM)
+hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                            const __grid_constant__ FewParams p) {
+  using L = FewLayout<MP>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t sB = smem_base + L::OFF_B, sA = smem_base + L::OFF_A;
+  float* factors = reinterpret_cast<float*>(smem + L::OFF_F);
+  const uint32_t bar_full = smem_base + L::OFF_BAR;
+  const uint32_t bar_empty = bar_full + L::STAGES * 8;
+  const uint32_t bar_tfull = bar_empty + L::STAGES * 8;
+  const uint32_t bar_tempty = bar_tfull + FEW_SLOTS * 8;
+  const uint32_t bar_ffull = bar_tempty + FEW_SLOTS * 8;
+  const uint32_t bar_xfull = bar_ffull + FEW_SLOTS * 8;
+  volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_TMEM_PTR);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_ABORT);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int S = p.cluster;
+  const int rank = static_cast<int>(cluster_ctarank());
+  // the cluster's slabs are first_slab, first_slab + step, ...; unit u of the cluster is k-block u % num_kb
+  // of its slab number u / num_kb; this CTA has the units [u_begin, u_end), never none: a cluster has a
+  // slab, and S is at most num_kb
+  const int first_slab = blockIdx.x / S, step = gridDim.x / S;
+  const int64_t all = static_cast<int64_t>((p.slabs - first_slab + step - 1) / step) * p.num_kb;
+  auto begin_of = [&](int c) { return all * c / S; };
+  auto owner_of = [&](int64_t u) { return static_cast<int>(((u + 1) * S - 1) / all); };   // CTA of unit u
+  const int64_t u_begin = begin_of(rank), u_end = begin_of(rank + 1);
+  const int64_t units = u_end - u_begin;
+  const int slab0 = first_slab + static_cast<int>(u_begin / p.num_kb) * step, kb0 = static_cast<int>(u_begin % p.num_kb);
+  // CTAs that send this one their part of the slab that it starts last
+  const int64_t last_start = (u_end - 1) / p.num_kb * p.num_kb;
+  const int senders = last_start >= u_begin ? owner_of(last_start + p.num_kb - 1) - rank : 0;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    for (int s = 0; s < L::STAGES; ++s) {
+      mbar_init(bar_full + s * 8, 1);
+      mbar_init(bar_empty + s * 8, 1);
+    }
+    for (int a = 0; a < FEW_SLOTS; ++a) {
+      mbar_init(bar_tfull + a * 8, 1);
+      mbar_init(bar_tempty + a * 8, 4);
+      mbar_init(bar_ffull + a * 8, 1);
+    }
+    for (int w = 0; w < 4; ++w) mbar_init(bar_xfull + w * 8, max(senders, 1));
+    mbar_fence_init();
+    fence_proxy_async_smem();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)), L::TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  cluster_sync();               // the partners' barriers are initialised
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr_smem;
+  grid_launch_dependents();     // the next kernel on the stream may begin its own prologue
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA producer
+    if (elect_one()) {
+      bool ok = true;
+      // ring fill: B before the dependency wait, A after it; the stages are empty at the start
+      const int fill = static_cast<int>(min(units, static_cast<int64_t>(L::STAGES)));
+      int slab = slab0, kb = kb0;
+      auto next = [&] {
+        if (++kb == p.num_kb) { kb = 0; slab += step; }
+      };
+      for (int i = 0; i < fill; ++i) {
+        mbar_arrive_expect_tx(bar_full + i * 8, L::A_BYTES + L::B_BYTES);
+        tma_load_2d(sB + i * L::B_BYTES, &tmB, bar_full + i * 8, kb * KB, slab * SLAB);
+        next();
+      }
+      const int slab_behind = slab, kb_behind = kb;
+      grid_dependency_wait();
+      kb = kb0;
+      for (int i = 0; i < fill; ++i) {
+        tma_load_2d(sA + i * L::A_BYTES, &tmA, bar_full + i * 8, kb * KB, 0);
+        next();
+      }
+      slab = slab_behind;
+      kb = kb_behind;
+      int s = fill == L::STAGES ? 0 : fill;
+      uint32_t phase = fill == L::STAGES ? 1 : 0;
+      for (int64_t u = fill; u < units; ++u) {
+        if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
+        mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
+        tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, kb * KB, slab * SLAB);
+        tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, kb * KB, 0);
+        next();
+        if (++s == L::STAGES) { s = 0; phase ^= 1; }
+      }
+      if (!ok) report_timeout(p.status, 11);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idesc = umma_idesc_e4m3(SLAB, MP);
+      int s = 0, slot = 0;
+      uint32_t phase = 0, slot_phase = 0;
+      bool ok = true;
+      for (int64_t u = 0; u < units; ++u) {
+        if (!mbar_wait(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag) || !mbar_wait(bar_full + s * 8, phase, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < KB / UMMA_K; ++k)
+          umma_e4m3<1>(tmem_base + slot * MP, umma_desc_k_sw128(sB + s * L::B_BYTES + k * UMMA_K),
+                       umma_desc_k_sw128(sA + s * L::A_BYTES + k * UMMA_K), idesc, k != 0 ? 1u : 0u);
+        umma_commit<1>(bar_empty + s * 8);
+        umma_commit<1>(bar_tfull + slot * 8);
+        if (++s == L::STAGES) { s = 0; phase ^= 1; }
+        if (++slot == FEW_SLOTS) { slot = 0; slot_phase ^= 1; }
+      }
+      if (!ok) report_timeout(p.status, 12);
+    }
+  } else if (warp == 6) {
+    // ---------------------------------------------------------------- factors a_scale * b_scale
+    // Eight units' scales are fetched at a time (units past the end repeat the last one), the next
+    // eight under the hand-over of these; the scales of a weight matrix do not wait for the kernel
+    // in front.
+    constexpr int PER = (MP + 31) / 32, AHEAD = FEW_SLOTS;
+    float fa[AHEAD][PER], fb[AHEAD];
+    int slab = slab0, kb = kb0;                  // of the next unit to fetch
+    int64_t left = units;
+    auto next = [&] {
+      if (--left <= 0) return;
+      if (++kb == p.num_kb) { kb = 0; slab += step; }
+    };
+    auto fetch_a = [&](float (&x)[PER], int at) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) x[i] = __ldg(p.sa + min(lane + 32 * i, p.M - 1) * p.sa_m + at * p.sa_k);
+    };
+    int first_kb[AHEAD];
+    if (!p.b_is_weights) grid_dependency_wait();
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      fb[j] = __ldg(p.sb + slab * p.sb_n + kb * p.sb_k);
+      first_kb[j] = kb;
+      next();
+    }
+    grid_dependency_wait();
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) fetch_a(fa[j], first_kb[j]);
+    uint32_t slot_phase = 0;
+    bool ok = true;
+    for (int64_t u = 0; u < units && ok; u += AHEAD, slot_phase ^= 1) {
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (u + j < units && ok) {
+          ok = mbar_wait(bar_tempty + j * 8, slot_phase ^ 1, abort_flag);
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (lane + 32 * i < MP) factors[j * MP + lane + 32 * i] = fa[j][i] * fb[j];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_ffull + j * 8);
+          fb[j] = __ldg(p.sb + slab * p.sb_n + kb * p.sb_k);
+          fetch_a(fa[j], kb);
+          next();
+        }
+      }
+    }
+    if (!ok && lane == 0) report_timeout(p.status, 14);
+  } else {
+    // ---------------------------------------------------------------- sums (warps 2..5)
+    const int q = warp & 3;
+    const int r = q * 32 + lane;                 // row of the slab = output column slab * 128 + r
+    const uint32_t t_mine = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    const uint32_t x_mine = smem_base + L::OFF_X + r * 4;
+    const float* x_local = reinterpret_cast<const float*>(smem + L::OFF_X) + r;
+    float* w_local = reinterpret_cast<float*>(smem + L::OFF_W) + r;
+    int slot = 0;
+    uint32_t slot_phase = 0;
+    bool ok = true;
+    grid_dependency_wait();                      // C may still be in use by the kernel in front
+    int slab = slab0, kb = kb0;
+    for (int64_t u = u_begin; u < u_end; slab += step, kb = 0) {
+      const int nkb = static_cast<int>(min(u_end - u, static_cast<int64_t>(p.num_kb - kb)));
+      uint64_t acc[MP / 2];
+#pragma unroll
+      for (int i = 0; i < MP / 2; ++i) acc[i] = 0;
+      for (int i = 0; i < nkb; ++i) {
+        ok = mbar_wait(bar_ffull + slot * 8, slot_phase, abort_flag) && mbar_wait(bar_tfull + slot * 8, slot_phase, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[MP / 16][16];
+#pragma unroll
+        for (int c = 0; c < MP / 16; ++c) tmem_ld_32x16(t_mine + slot * MP + c * 16, v[c]);
+        tmem_wait_ld();
+        const float4* f4 = reinterpret_cast<const float4*>(factors + slot * MP);
+#pragma unroll
+        for (int c = 0; c < MP / 4; ++c) {
+          const float4 f = f4[c];
+          const uint32_t* t = &v[c / 4][c % 4 * 4];
+          fma2(acc[2 * c], t[0], t[1], pack2(f.x, f.y));
+          fma2(acc[2 * c + 1], t[2], t[3], pack2(f.z, f.w));
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_tempty + slot * 8);    // sums and factors are in registers
+        if (++slot == FEW_SLOTS) { slot = 0; slot_phase ^= 1; }
+      }
+      if (!ok) break;
+      if (kb > 0) {
+        // the slab was started by another CTA: send the sums there; warp q hears from warps q alone
+        const int starter = owner_of(u - kb);
+        const uint32_t dst = mapa(x_mine + (rank - starter - 1) * (MP * SLAB * 4), starter);
+#pragma unroll
+        for (int m = 0; m < MP; ++m) {
+          const float2 two = unpack2(acc[m / 2]);
+          if (m < p.M) st_cluster_f32(dst + m * (SLAB * 4), m & 1 ? two.y : two.x);
+        }
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive_release_cluster(mapa(bar_xfull + q * 8, starter));
+        u += nkb;
+        continue;
+      }
+      if (nkb < p.num_kb) {
+        ok = mbar_wait_acquire_cluster(bar_xfull + q * 8, 0, abort_flag);
+        if (!ok) break;
+      }
+      u += nkb;
+      const int from = nkb < p.num_kb ? senders : 0;
+      const int n = slab * SLAB + r;
+      // sixteen rows at a time through shared memory (each thread its own column), so that the
+      // epilogue is a short loop: unrolled over the accumulators it would not fit the instruction cache
+#pragma unroll
+      for (int c16 = 0; c16 < MP; c16 += 16) {
+        if (c16 >= p.M) break;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float2 two = unpack2(acc[(c16 + i) / 2]);
+          w_local[i * SLAB] = i & 1 ? two.y : two.x;
+        }
+        for (int i = 0; i < 16 && c16 + i < p.M; i += 4) {
+          float v[4];                             // rows past the last are read (from this buffer) and not used
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = w_local[(i + j) * SLAB];
+          for (int c = 0; c < from; ++c)          // in k order
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += x_local[(c * MP + c16 + i + j) * SLAB];
+          const int rows = min(4, p.M - c16 - i);
+          if (p.epilogue == HB_EPI_SWIGLU) {      // columns interleave (gate, up): two neighbouring lanes
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = silu(v[j]) * __shfl_down_sync(0xffffffffu, v[j], 1);
+          } else if (p.epilogue == HB_EPI_GELU) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = gelu_erf(v[j]);
+          } else if (p.epilogue == HB_EPI_RESIDUAL) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < rows && n < p.N) v[j] += __bfloat162float(p.R[(c16 + i + j) * p.ldr + n]);
+          }
+          const bool mine = n < p.N && !(p.epilogue == HB_EPI_SWIGLU && (r & 1));
+          __nv_bfloat16* dst = p.C + (c16 + i) * p.ldc + (p.epilogue == HB_EPI_SWIGLU ? n >> 1 : n);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < rows && mine) dst[j * p.ldc] = __float2bfloat16_rn(v[j]);
+        }
+      }
+    }
+    if (!ok && lane == 0) report_timeout(p.status, 13);
+  }
+
+  // no CTA may leave while a partner can still write to its shared memory
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, L::TMEM_COLS);
+  }
+}
+
+template <int MP>
+hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
+  using L = FewLayout<MP>;
+  auto kern = hb_matmul_scaled_few_kernel<MP>;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(FEW_THREADS);
+  cfg.dynamicSmemBytes = L::DYN_BYTES;
+  cfg.stream = ctx->stream;
+  cfg.attrs = attr;
+  // clusters of S CTAs that can run at once, one CTA per SM
+  static int resident[64][FEW_MAX_CLUSTER + 1] = {};
+  int* most = resident[ctx->device & 63];
+  if (!most[1]) {
+    HB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN_BYTES));
+    for (int c = FEW_MAX_CLUSTER; c >= 1; --c) {
+      attr[0].val.clusterDim.x = c;
+      cfg.gridDim = dim3(ctx->sm_count / c * c);
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
+      most[c] = n < ctx->sm_count / c ? n : ctx->sm_count / c;
+      if (c == 1 && most[c] < 1) most[c] = ctx->sm_count;
+    }
+  }
+  CUtensorMap tmA, tmB;
+  uint64_t dims[2] = {(uint64_t)g.K, (uint64_t)g.M}, pitch[1] = {(uint64_t)g.lda};
+  uint32_t box[2] = {KB, MP};
+  hb_status st = hb_make_tensor_map(ctx, &tmA, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, g.A, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st != HB_OK) return st;
+  dims[1] = (uint64_t)g.N; pitch[0] = (uint64_t)g.ldb; box[1] = SLAB;
+  if ((st = hb_make_tensor_map(ctx, &tmB, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, g.B, dims, pitch, box, CU_TENSOR_MAP_SWIZZLE_128B)) != HB_OK) return st;
+  FewParams p;
+  memset(&p, 0, sizeof(p));
+  p.sa = g.sa; p.sb = g.sb; p.C = g.C; p.R = g.R;
+  p.ldc = g.ldc; p.ldr = g.ldr;
+  p.sa_m = g.sa_m; p.sa_k = g.sa_k; p.sb_n = g.sb_n; p.sb_k = g.sb_k;
+  p.M = (int)g.M; p.N = (int)g.N;
+  p.num_kb = (int)((g.K + KB - 1) / KB);
+  p.slabs = (int)((g.N + SLAB - 1) / SLAB);
+  p.epilogue = g.epilogue;
+  p.b_is_weights = g.b_is_weights;
+  p.status = ctx->d_status;
+  // k-blocks that the busiest CTA streams
+  double best = 0;
+  for (int c = 1; c <= FEW_MAX_CLUSTER && c <= p.num_kb; ++c) {
+    if (most[c] < 1) continue;
+    const int64_t clusters = p.slabs < most[c] ? p.slabs : most[c];
+    const double cost = (double)((p.slabs + clusters - 1) / clusters) * p.num_kb / c;
+    if (p.cluster == 0 || cost < best) { best = cost; p.cluster = c; }
+  }
+  const int clusters = p.slabs < most[p.cluster] ? p.slabs : most[p.cluster];
+  attr[0].val.clusterDim.x = p.cluster;
+  cfg.gridDim = dim3((unsigned)(clusters * p.cluster));
+  cfg.numAttrs = g.b_is_weights ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tmA, tmB, p);
+  if (e != cudaSuccess) { cudaGetLastError(); return hb_check_cuda(ctx, e, "matmul_scaled launch"); }
+  ctx->launches++;
+  return HB_OK;
+}
+
 hb_status launch(hb_ctx* ctx, const ScaledArgs& g) {
+  if (g.M <= FEW_MAX_M)
+    return g.M <= 16 ? launch_few<16>(ctx, g) : g.M <= 32 ? launch_few<32>(ctx, g) : launch_few<64>(ctx, g);
   if (g.M > 128 && g.N > 128) return launch_tile<true, 256, 5>(ctx, g);
   return launch_tile<false, 128, 4>(ctx, g);
 }
