@@ -369,8 +369,8 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       tile_coords(tile, p, tm, tn);
       sa = p.sa + min(tm * L::BM + rank * 128 + q * 32 + lane, p.M - 1) * p.sa_m;
       sb = p.sb + min((tn * BN + h * HALF) / KB, p.nblocks - 1) * p.sb_n;
-      fa = __ldg(sa);
-      fb = __ldg(sb);
+      fa = *sa;
+      fb = *sb;
     };
     if (unit < num_tiles) first_scales(unit);
     for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
@@ -380,8 +380,8 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       for (int kb = 0; kb < p.num_kb; ++kb) {
         const uint64_t f = pack2(fa * fb, fa * fb);
         if (kb + 1 < p.num_kb) {                     // the next block's scales arrive under this block's sums
-          fa = __ldg(sa + (kb + 1) * p.sa_k);
-          fb = __ldg(sb + (kb + 1) * p.sb_k);
+          fa = sa[(kb + 1) * p.sa_k];
+          fb = sb[(kb + 1) * p.sb_k];
         }
         if (!mbar_wait(bar_tfull + slot * 8, slot_phase, abort_flag)) { ok = false; break; }
         tc_fence_after();
@@ -523,15 +523,12 @@ hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g) {
 // distributed shared memory, as the first thing that a CTA finishes; the starter comes to that slab
 // last, finds them there and adds them in k order: the same bits every run, nothing waits in
 // practice, and there is no scratch and no counter in global memory that launches could share.
-// For up to 16 rows a CTA takes less than half an SM, so that the next launch on the stream can set
-// itself up beside this one.  With HB_MATMUL_WEIGHTS_B it also fills its ring with B before the kernel
-// in front has finished (programmatic dependent launch); what depends on that kernel comes after the
-// wait.
+// With HB_MATMUL_WEIGHTS_B a CTA fills its ring with B before the kernel in front has finished
+// (programmatic dependent launch); what depends on that kernel comes after the wait.
 // ------------------------------------------------------------------------------------
 constexpr int FEW_MAX_M = 64;
 constexpr int FEW_THREADS = 224;                 // TMA, MMA, four warps of sums, factors
 constexpr int FEW_SLOTS = 8;
-constexpr int FEW_MAX_CLUSTER = 4;
 constexpr int SLAB = 128;
 
 struct FewParams {
@@ -549,12 +546,12 @@ struct FewParams {
 template <int MP>
 struct FewLayout {
   static constexpr int A_BYTES = MP * KB, B_BYTES = SLAB * KB;
-  static constexpr int CTAS_PER_SM = MP <= 16 ? 2 : 1;
+  static constexpr int MAX_CLUSTER = MP <= 16 ? 6 : 4;                    // the sums received have to fit beside the ring
   static constexpr uint32_t TMEM_COLS = FEW_SLOTS * MP;                   // 128, 256 or 512
   static constexpr int F_BYTES = FEW_SLOTS * MP * 4;                      // factors: [slot][MP] fp32
-  static constexpr int X_BYTES = (FEW_MAX_CLUSTER - 1) * MP * SLAB * 4;   // sums received: [sender][row of A][128] fp32
+  static constexpr int X_BYTES = (MAX_CLUSTER - 1) * MP * SLAB * 4;   // sums received: [sender][row of A][128] fp32
   static constexpr int W_BYTES = 16 * SLAB * 4;                           // sixteen rows on their way out
-  static constexpr int STAGES = (227 * 1024 / CTAS_PER_SM - 4096 - F_BYTES - X_BYTES - W_BYTES) / (A_BYTES + B_BYTES);
+  static constexpr int STAGES = (227 * 1024 - 4096 - F_BYTES - X_BYTES - W_BYTES) / (A_BYTES + B_BYTES);
   static constexpr int OFF_B = 0;
   static constexpr int OFF_A = OFF_B + STAGES * B_BYTES;
   static constexpr int OFF_F = OFF_A + STAGES * A_BYTES;
@@ -564,7 +561,7 @@ struct FewLayout {
   static constexpr int OFF_TMEM_PTR = OFF_BAR + (2 * STAGES + 3 * FEW_SLOTS + 4) * 8;
   static constexpr int OFF_ABORT = OFF_TMEM_PTR + 4;
   static constexpr int DYN_BYTES = OFF_ABORT + 4 + 1024;
-  static_assert(CTAS_PER_SM * (DYN_BYTES + 1024) <= 228 * 1024 && STAGES >= 3, "ring does not fit shared memory");
+  static_assert(DYN_BYTES <= 227 * 1024 && STAGES >= 4, "ring does not fit shared memory");
 };
 
 // Arrive on / wait for a barrier when the data it stands for crossed between CTAs of the cluster.
@@ -590,7 +587,7 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
 }
 
 template <int MP>
-__global__ void __launch_bounds__(FEW_THREADS, FewLayout<MP>::CTAS_PER_SM)
+__global__ void __launch_bounds__(FEW_THREADS, 1)
 hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                             const __grid_constant__ FewParams p) {
   using L = FewLayout<MP>;
@@ -728,13 +725,13 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     };
     auto fetch_a = [&](float (&x)[PER], int at) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) x[i] = __ldg(p.sa + min(lane + 32 * i, p.M - 1) * p.sa_m + at * p.sa_k);
+      for (int i = 0; i < PER; ++i) x[i] = p.sa[min(lane + 32 * i, p.M - 1) * p.sa_m + at * p.sa_k];
     };
     int first_kb[AHEAD];
     if (!p.b_is_weights) grid_dependency_wait();
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      fb[j] = __ldg(p.sb + slab * p.sb_n + kb * p.sb_k);
+      fb[j] = p.sb[slab * p.sb_n + kb * p.sb_k];
       first_kb[j] = kb;
       next();
     }
@@ -753,7 +750,7 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
             if (lane + 32 * i < MP) factors[j * MP + lane + 32 * i] = fa[j][i] * fb[j];
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_ffull + j * 8);
-          fb[j] = __ldg(p.sb + slab * p.sb_n + kb * p.sb_k);
+          fb[j] = p.sb[slab * p.sb_n + kb * p.sb_k];
           fetch_a(fa[j], kb);
           next();
         }
@@ -886,11 +883,11 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   // clusters of S CTAs that can run at once, one CTA per SM
-  static int resident[64][FEW_MAX_CLUSTER + 1] = {};
+  static int resident[64][L::MAX_CLUSTER + 1] = {};
   int* most = resident[ctx->device & 63];
   if (!most[1]) {
     HB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN_BYTES));
-    for (int c = FEW_MAX_CLUSTER; c >= 1; --c) {
+    for (int c = L::MAX_CLUSTER; c >= 1; --c) {
       attr[0].val.clusterDim.x = c;
       cfg.gridDim = dim3(ctx->sm_count / c * c);
       cfg.numAttrs = 1;
@@ -920,7 +917,7 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
   p.status = ctx->d_status;
   // k-blocks that the busiest CTA streams
   double best = 0;
-  for (int c = 1; c <= FEW_MAX_CLUSTER && c <= p.num_kb; ++c) {
+  for (int c = 1; c <= L::MAX_CLUSTER && c <= p.num_kb; ++c) {
     if (most[c] < 1) continue;
     const int64_t clusters = p.slabs < most[c] ? p.slabs : most[c];
     const double cost = (double)((p.slabs + clusters - 1) / clusters) * p.num_kb / c;
