@@ -95,22 +95,29 @@ __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __e
 constexpr uint32_t umma_idesc_e4m3(int m, int n) {
   return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
+// Shared-memory descriptor of a K-major tile with 128-byte rows and 128-byte swizzle (as
+// umma_desc_k_sw128), in two words: the low one carries the address and moves by plain addition.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
+// One k-block: four MMAs of K = 32, the first of them overwriting D.  Executed by a whole converged
+// warp -- one thread issues -- so that the operands stay in uniform registers; a loop inside a
+// one-thread branch has to move every operand there and took some 500 clocks per k-block.
 template <int CTA_GROUP>
-__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CTA_GROUP == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+__device__ __forceinline__ void umma_kblock(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+#define HB_UMMA(GROUP, K, ACC)                                                                                            \
+  asm volatile(                                                                                                           \
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t" \
+      "tcgen05.mma.cta_group::" #GROUP ".kind::f8f6f4 [%0], da, db, %4, p;\n\t}\n" ::"r"(d_tmem),                          \
+      "r"(a_lo + (K) * (UMMA_K >> 4)), "r"(b_lo + (K) * (UMMA_K >> 4)), "r"(DESC_HI), "r"(idesc), "n"(ACC)                  \
+      : "memory")
+  if constexpr (CTA_GROUP == 1) {
+    HB_UMMA(1, 0, 0); HB_UMMA(1, 1, 1); HB_UMMA(1, 2, 1); HB_UMMA(1, 3, 1);
+  } else {
+    HB_UMMA(2, 0, 0); HB_UMMA(2, 1, 1); HB_UMMA(2, 2, 1); HB_UMMA(2, 3, 1);
+  }
+#undef HB_UMMA
+  static_assert(KB / UMMA_K == 4, "four steps");
 }
-
 // Two sums at once: acc += t * f.  Volatile like the tensor-memory load and the wait for it, so that it stays behind both.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t t0, uint32_t t1, uint64_t f) {
   asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(t0), "r"(t1), "l"(f));
@@ -288,9 +295,8 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
   const int num_tiles = p.tiles_m * p.tiles_n;
   if (warp < EPI_WARP0) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_FEW));
-  if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (elect_one()) {
+    if (warp == 0) {
+      // ---------------------------------------------------------- TMA producer
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -300,54 +306,56 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
         const int m0 = tm * L::BM + rank * 128, n0 = tn * BN + rank * L::B_ROWS;
         for (int kb = 0; kb < p.num_kb; ++kb) {
           if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
-          if constexpr (PAIR) {
-            const uint32_t full_leader = mapa(bar_full + s * 8, 0);
-            if (rank == 0) mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
-            else mbar_arrive_expect_tx_cluster(full_leader, L::A_BYTES + L::B_BYTES);
-            tma_load_2d_pair(sA + s * L::A_BYTES, &tmA, full_leader, kb * KB, m0);
-            tma_load_2d_pair(sB + s * L::B_BYTES, &tmB, full_leader, kb * KB, n0);
-          } else {
-            mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
-            tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, kb * KB, m0);
-            tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, kb * KB, n0);
+          if (elect_one()) {
+            if constexpr (PAIR) {
+              const uint32_t full_leader = mapa(bar_full + s * 8, 0);
+              if (rank == 0) mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
+              else mbar_arrive_expect_tx_cluster(full_leader, L::A_BYTES + L::B_BYTES);
+              tma_load_2d_pair(sA + s * L::A_BYTES, &tmA, full_leader, kb * KB, m0);
+              tma_load_2d_pair(sB + s * L::B_BYTES, &tmB, full_leader, kb * KB, n0);
+            } else {
+              mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
+              tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, kb * KB, m0);
+              tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, kb * KB, n0);
+            }
           }
+          __syncwarp();
           if (++s == STAGES) { s = 0; phase ^= 1; }
         }
       }
-      if (!ok) report_timeout(p.status, 1);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (of a pair: the leader)
-    if (rank == 0 && elect_one()) {
+      if (!ok && lane == 0) report_timeout(p.status, 1);
+    } else if (warp == 1 && rank == 0) {
+      // ---------------------------------------------------------- MMA issuer (of a pair: the leader)
       constexpr uint32_t idesc = umma_idesc_e4m3(L::BM, BN);
+      const uint32_t a_lo = desc_lo(sA), b_lo = desc_lo(sB);
       int s = 0, slot = 0;
       uint32_t phase = 0, slot_phase = 0;
       bool ok = true;
       for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
         for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_spin(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag) || !mbar_wait_spin(bar_full + s * 8, phase, abort_flag)) {
+          // the data first: a slot is what comes late, and each wait costs about a hundred clocks
+          if (!mbar_wait_spin(bar_full + s * 8, phase, abort_flag) || !mbar_wait_spin(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < KB / UMMA_K; ++k)
-            umma_e4m3<GROUP>(tmem_base + slot * BN, umma_desc_k_sw128(sA + s * L::A_BYTES + k * UMMA_K),
-                             umma_desc_k_sw128(sB + s * L::B_BYTES + k * UMMA_K), idesc, k != 0 ? 1u : 0u);
-          if constexpr (PAIR) {
-            umma_commit_pair_mcast(bar_empty + s * 8, 3);
-            umma_commit_pair_mcast(bar_tfull + slot * 8, 3);
-          } else {
-            umma_commit<1>(bar_empty + s * 8);
-            umma_commit<1>(bar_tfull + slot * 8);
+          if (elect_one()) {
+            umma_kblock<GROUP>(tmem_base + slot * BN, a_lo + s * (L::A_BYTES >> 4), b_lo + s * (L::B_BYTES >> 4), idesc);
+            if constexpr (PAIR) {
+              umma_commit_pair_mcast(bar_tfull + slot * 8, 3);
+              umma_commit_pair_mcast(bar_empty + s * 8, 3);
+            } else {
+              umma_commit<1>(bar_tfull + slot * 8);
+              umma_commit<1>(bar_empty + s * 8);
+            }
           }
+          __syncwarp();
           if (++s == STAGES) { s = 0; phase ^= 1; }
           if (++slot == L::SLOTS) { slot = 0; slot_phase ^= 1; }
         }
       }
-      if (!ok) report_timeout(p.status, 2);
+      if (!ok && lane == 0) report_timeout(p.status, 2);
     }
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_MANY));
     // ------------------------------------------------------------ sums (warps 4..11)
@@ -652,64 +660,68 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
-    if (elect_one()) {
-      bool ok = true;
-      // ring fill: B before the dependency wait, A after it; the stages are empty at the start
-      const int fill = static_cast<int>(min(units, static_cast<int64_t>(L::STAGES)));
-      int slab = slab0, kb = kb0;
-      auto next = [&] {
-        if (++kb == p.num_kb) { kb = 0; slab += step; }
-      };
-      for (int i = 0; i < fill; ++i) {
+    bool ok = true;
+    // ring fill: B before the dependency wait, A after it; the stages are empty at the start
+    const int fill = static_cast<int>(min(units, static_cast<int64_t>(L::STAGES)));
+    int slab = slab0, kb = kb0;
+    auto next = [&] {
+      if (++kb == p.num_kb) { kb = 0; slab += step; }
+    };
+    for (int i = 0; i < fill; ++i) {
+      if (elect_one()) {
         mbar_arrive_expect_tx(bar_full + i * 8, L::A_BYTES + L::B_BYTES);
         tma_load_2d(sB + i * L::B_BYTES, &tmB, bar_full + i * 8, kb * KB, slab * SLAB);
-        next();
       }
-      const int slab_behind = slab, kb_behind = kb;
-      grid_dependency_wait();
-      kb = kb0;
-      for (int i = 0; i < fill; ++i) {
-        tma_load_2d(sA + i * L::A_BYTES, &tmA, bar_full + i * 8, kb * KB, 0);
-        next();
-      }
-      slab = slab_behind;
-      kb = kb_behind;
-      int s = fill == L::STAGES ? 0 : fill;
-      uint32_t phase = fill == L::STAGES ? 1 : 0;
-      for (int64_t u = fill; u < units; ++u) {
-        if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
+      __syncwarp();
+      next();
+    }
+    const int slab_behind = slab, kb_behind = kb;
+    grid_dependency_wait();
+    kb = kb0;
+    for (int i = 0; i < fill; ++i) {
+      if (elect_one()) tma_load_2d(sA + i * L::A_BYTES, &tmA, bar_full + i * 8, kb * KB, 0);
+      __syncwarp();
+      next();
+    }
+    slab = slab_behind;
+    kb = kb_behind;
+    int s = fill == L::STAGES ? 0 : fill;
+    uint32_t phase = fill == L::STAGES ? 1 : 0;
+    for (int64_t u = fill; u < units; ++u) {
+      if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
+      if (elect_one()) {
         mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
         tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, kb * KB, slab * SLAB);
         tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, kb * KB, 0);
-        next();
-        if (++s == L::STAGES) { s = 0; phase ^= 1; }
       }
-      if (!ok) report_timeout(p.status, 11);
+      __syncwarp();
+      next();
+      if (++s == L::STAGES) { s = 0; phase ^= 1; }
     }
+    if (!ok && lane == 0) report_timeout(p.status, 11);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
-    if (elect_one()) {
-      constexpr uint32_t idesc = umma_idesc_e4m3(SLAB, MP);
-      int s = 0, slot = 0;
-      uint32_t phase = 0, slot_phase = 0;
-      bool ok = true;
-      for (int64_t u = 0; u < units; ++u) {
-        if (!mbar_wait(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag) || !mbar_wait(bar_full + s * 8, phase, abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < KB / UMMA_K; ++k)
-          umma_e4m3<1>(tmem_base + slot * MP, umma_desc_k_sw128(sB + s * L::B_BYTES + k * UMMA_K),
-                       umma_desc_k_sw128(sA + s * L::A_BYTES + k * UMMA_K), idesc, k != 0 ? 1u : 0u);
-        umma_commit<1>(bar_empty + s * 8);
-        umma_commit<1>(bar_tfull + slot * 8);
-        if (++s == L::STAGES) { s = 0; phase ^= 1; }
-        if (++slot == FEW_SLOTS) { slot = 0; slot_phase ^= 1; }
+    constexpr uint32_t idesc = umma_idesc_e4m3(SLAB, MP);
+    const uint32_t a_lo = desc_lo(sA), b_lo = desc_lo(sB);
+    int s = 0, slot = 0;
+    uint32_t phase = 0, slot_phase = 0;
+    bool ok = true;
+    for (int64_t u = 0; u < units; ++u) {
+      if (!mbar_wait(bar_full + s * 8, phase, abort_flag) || !mbar_wait(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag)) {
+        ok = false;
+        break;
       }
-      if (!ok) report_timeout(p.status, 12);
+      tc_fence_after();
+      if (elect_one()) {
+        umma_kblock<1>(tmem_base + slot * MP, b_lo + s * (L::B_BYTES >> 4), a_lo + s * (L::A_BYTES >> 4), idesc);
+        umma_commit<1>(bar_tfull + slot * 8);
+        umma_commit<1>(bar_empty + s * 8);
+      }
+      __syncwarp();
+      if (++s == L::STAGES) { s = 0; phase ^= 1; }
+      if (++slot == FEW_SLOTS) { slot = 0; slot_phase ^= 1; }
     }
+    if (!ok && lane == 0) report_timeout(p.status, 12);
   } else if (warp == 6) {
     // ---------------------------------------------------------------- factors a_scale * b_scale
     // Eight units' scales are fetched at a time (units past the end repeat the last one), the next
@@ -936,8 +948,19 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
 hb_status launch(hb_ctx* ctx, const ScaledArgs& g) {
   if (g.M <= FEW_MAX_M)
     return g.M <= 16 ? launch_few<16>(ctx, g) : g.M <= 32 ? launch_few<32>(ctx, g) : launch_few<64>(ctx, g);
-  if (g.M > 128 && g.N > 128) return launch_tile<true, 256, 5>(ctx, g);
-  return launch_tile<false, 128, 4>(ctx, g);
+  // The tile whose waves take the least time.  A k-block costs, with one wave on the GPU (K = 4096,
+  // microseconds): 0.47 for 256 x 256 on a CTA pair, 0.36 for 256 x 128 on a pair, 0.50 for 128 x 256 on one
+  // CTA.  Measured, in that order: 512 x 6144 19.4 / 23.0 / 20.2 us, 512 x 4096 18.3 / 13.8 / 19.3, 128 x
+  // 28672 34.3 / 41.5 / 25.8, 4096 x 4096 65 / 81 / 70.
+  const auto cost = [&](int64_t bm, int64_t bn, int64_t at_once, double kblock) {
+    const int64_t tiles = (g.M + bm - 1) / bm * ((g.N + bn - 1) / bn);
+    return (double)((tiles + at_once - 1) / at_once) * kblock;
+  };
+  const double pair_wide = cost(256, 256, ctx->sm_count / 2, 0.47), pair_narrow = cost(256, 128, ctx->sm_count / 2, 0.36),
+               one = cost(128, 256, ctx->sm_count, 0.50);
+  if (pair_wide <= pair_narrow && pair_wide <= one) return launch_tile<true, 256, 5>(ctx, g);
+  if (pair_narrow <= one) return launch_tile<true, 128, 6>(ctx, g);
+  return launch_tile<false, 256, 3>(ctx, g);
 }
 
 hb_status decode(hb_ctx* ctx, const hb_tensor* A, const hb_tensor* sa, const hb_tensor* B, const hb_tensor* sb,
