@@ -16,6 +16,7 @@
 // what the launch holds).
 // Algorithmic traffic per launch: M*K + N*K + 2*M*N bytes and the scales; work 2*M*N*K flop at the
 // 8-bit tensor rate (twice that of bf16).
+#include <math.h>
 #include <string.h>
 
 #include <new>
@@ -54,8 +55,8 @@ struct TileParams {
   int64_t ldc, ldr, sa_m, sa_k, sb_n, sb_k;
   int M, N, num_kb, nblocks;     // nblocks: 128-wide blocks of B
   int tiles_m, tiles_n, raster_group;
-  int epilogue;
   int tma_store;
+  int split;                     // CTAs that share a tile's k-blocks
   int32_t* status;
 };
 
@@ -66,19 +67,24 @@ constexpr int STAGE_BUF_BYTES = 32 * 64;
 constexpr int STAGE_BUFS = 4;
 constexpr int STAGE_BYTES = EPI_WARPS * STAGE_BUFS * STAGE_BUF_BYTES;
 
-template <bool PAIR, int BN, int STAGES>
+constexpr int SPLIT_MAX = 4;       // CTAs that may share a tile's k-blocks (its sums travel in pieces of sixteen columns)
+// PAIR: two CTAs share a tile of 256 rows.  SPLIT: a cluster of CTAs shares the k-blocks of one tile.
+enum { TILE_ONE = 0, TILE_PAIR = 1, TILE_SPLIT = 2 };
+
+template <int KIND, int BN, int STAGES>
 struct TileLayout {
+  static constexpr bool PAIR = KIND == TILE_PAIR;
   static constexpr int BM = PAIR ? 256 : 128;
   static constexpr int B_ROWS = PAIR ? BN / 2 : BN;      // rows of B that one CTA loads
   static constexpr int A_BYTES = 128 * KB;
   static constexpr int B_BYTES = B_ROWS * KB;
-  static constexpr int SLOTS = BN == 256 ? 2 : 4;
-  static constexpr uint32_t TMEM_COLS = SLOTS * BN;      // 512, 512 or 256: a power of two
+  static constexpr int SLOTS = 512 / BN;
+  static constexpr uint32_t TMEM_COLS = 512;
   static constexpr int OFF_A = 0;
   static constexpr int OFF_B = OFF_A + STAGES * A_BYTES;
   static constexpr int OFF_STAGE = OFF_B + STAGES * B_BYTES;
   static constexpr int OFF_BAR = OFF_STAGE + STAGE_BYTES;
-  static constexpr int NUM_BARS = 2 * STAGES + 2 * SLOTS;   // full, empty, tfull, tempty
+  static constexpr int NUM_BARS = 2 * STAGES + 2 * SLOTS + 2 * EPI_WARPS;   // full, empty, tfull, tempty, xready, xfull
   static constexpr int OFF_TMEM_PTR = OFF_BAR + NUM_BARS * 8;
   static constexpr int OFF_ABORT = OFF_TMEM_PTR + 4;
   static constexpr int TOTAL = OFF_ABORT + 4;
@@ -168,16 +174,18 @@ __device__ __forceinline__ void put_chunk(const TileParams& p, uint32_t stage, i
   }
 }
 
-// The accumulators of one thread (row `row0 + lane`, HALF columns from col0 on) -> C.
-template <int HALF>
+// The accumulators of one thread (row `row0 + lane`, HALF columns from col0 on) -> C.  The epilogue is a
+// template argument here and in the kernels: this code runs once per tile, and what it takes is mostly
+// the fetching of its instructions.
+template <int EPI, int HALF>
 __device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMap* tmC, uint32_t stage, int lane, int row0,
                                            int col0, const uint64_t (&acc)[HALF / 2]) {
   if (p.tma_store) {
     if (lane == 0) tma_store_wait_read<0>();     // the last tile's stores have read the buffers
     __syncwarp();
   }
-  const bool swiglu = HALF >= 64 && p.epilogue == HB_EPI_SWIGLU;
-  if (swiglu) {
+  constexpr bool swiglu = EPI == HB_EPI_SWIGLU;
+  if constexpr (swiglu) {
     // columns interleave (gate, up): 64 sums give 32 outputs
 #pragma unroll
     for (int c = 0; c < HALF / 64; ++c) {
@@ -200,10 +208,11 @@ __device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMa
         f[2 * j + 1] = v.y;
       }
       const int col = col0 + c * 32;
-      if (p.epilogue == HB_EPI_GELU) {
+      if constexpr (EPI == HB_EPI_GELU) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
-      } else if (p.epilogue == HB_EPI_RESIDUAL && row0 + lane < p.M) {
+      }
+      if (EPI == HB_EPI_RESIDUAL && row0 + lane < p.M) {
         const __nv_bfloat16* r = p.R + static_cast<int64_t>(row0 + lane) * p.ldr + col;
         if ((p.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(p.R) & 15) == 0 && col + 32 <= p.N) {
 #pragma unroll
@@ -242,11 +251,85 @@ __device__ __forceinline__ void report_timeout(int32_t* status, int what) {
   if (status) { atomicCAS(status, 0, HB_ERR_TIMEOUT); status[1] = HB_KTAG_SCALED; status[2] = what; }
 }
 
-template <bool PAIR, int BN, int STAGES>
+// Arrive on / wait for a barrier when the data it stands for crossed between CTAs of the cluster.
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < HB_SPIN_LIMIT; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((i & 1023u) == 1023u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  return false;
+}
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+
+// Sixteen finished sums of row `row` from column col0 on: epilogue, one rounding, stores of the row's own
+// bytes (a tile that is split is one of few, and its output small).
+template <int EPI>
+__device__ __forceinline__ void put16(const TileParams& p, int row, int col0, float (&f)[16]) {
+  if (row >= p.M) return;
+  constexpr bool swiglu = EPI == HB_EPI_SWIGLU;
+  constexpr int OUT = swiglu ? 8 : 16;
+  const int first = swiglu ? col0 >> 1 : col0, ncols = swiglu ? p.N >> 1 : p.N;
+  if constexpr (swiglu) {                          // columns interleave (gate, up)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = silu(f[2 * j]) * f[2 * j + 1];
+  }
+  if constexpr (EPI == HB_EPI_GELU) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = gelu_erf(f[j]);
+  }
+  if constexpr (EPI == HB_EPI_RESIDUAL) {
+    const __nv_bfloat16* r = p.R + static_cast<int64_t>(row) * p.ldr + first;
+    if (first + 16 <= ncols && (reinterpret_cast<uintptr_t>(r) & 15) == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4 rv = reinterpret_cast<const uint4*>(r)[h];
+        const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[8 * h + 2 * j] += __uint_as_float(rw[j] << 16);
+          f[8 * h + 2 * j + 1] += __uint_as_float(rw[j] & 0xffff0000u);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (first + j < ncols) f[j] += __bfloat162float(r[j]);
+    }
+  }
+  __nv_bfloat16* dst = p.C + static_cast<int64_t>(row) * p.ldc + first;
+  if (first + OUT <= ncols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+#pragma unroll
+    for (int h = 0; h < OUT / 8; ++h)
+      reinterpret_cast<uint4*>(dst)[h] = make_uint4(pack_bf16x2(f[8 * h], f[8 * h + 1]), pack_bf16x2(f[8 * h + 2], f[8 * h + 3]),
+                                                    pack_bf16x2(f[8 * h + 4], f[8 * h + 5]), pack_bf16x2(f[8 * h + 6], f[8 * h + 7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < OUT; ++j)
+      if (first + j < ncols) dst[j] = __float2bfloat16_rn(f[j]);
+  }
+}
+
+template <int KIND, int BN, int STAGES, int EPI>
 __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC,
                                                  const TileParams& p) {
-  using L = TileLayout<PAIR, BN, STAGES>;
-  constexpr int GROUP = PAIR ? 2 : 1;
+  using L = TileLayout<KIND, BN, STAGES>;
+  constexpr bool PAIR = KIND == TILE_PAIR, SPLIT = KIND == TILE_SPLIT;
+  constexpr int GROUP = PAIR ? 2 : 1;             // CTAs that one MMA spans
   constexpr int HALF = BN / 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -257,14 +340,22 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
   const uint32_t bar_empty = bar_full + STAGES * 8;
   const uint32_t bar_tfull = bar_empty + STAGES * 8;
   const uint32_t bar_tempty = bar_tfull + L::SLOTS * 8;
+  const uint32_t bar_xready = bar_tempty + L::SLOTS * 8;
+  const uint32_t bar_xfull = bar_xready + EPI_WARPS * 8;
   volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_TMEM_PTR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_ABORT);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
-  const int unit = blockIdx.x / GROUP;               // CTA or pair
-  const int num_units = gridDim.x / GROUP;
+  // CTA, pair or cluster; a split tile has a cluster of its own, whose CTAs take a contiguous share of
+  // the k-blocks each (never none: there are at least as many)
+  const int together = SPLIT ? p.split : GROUP;
+  const int unit = blockIdx.x / together;
+  const int num_units = gridDim.x / together;
+  const int part = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
+  const int kb_begin = SPLIT ? static_cast<int>(static_cast<int64_t>(p.num_kb) * part / p.split) : 0;
+  const int kb_end = SPLIT ? static_cast<int>(static_cast<int64_t>(p.num_kb) * (part + 1) / p.split) : p.num_kb;
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -276,6 +367,11 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       mbar_init(bar_tfull + a * 8, 1);
       mbar_init(bar_tempty + a * 8, EPI_WARPS * GROUP);
     }
+    if constexpr (SPLIT)
+      for (int w = 0; w < EPI_WARPS; ++w) {
+        mbar_init(bar_xready + w * 8, p.split);
+        mbar_init(bar_xfull + w * 8, p.split);
+      }
     mbar_fence_init();
     fence_proxy_async_smem();
     tma_prefetch_desc(&tmA);
@@ -286,7 +382,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
     tmem_relinquish<GROUP>();
   }
   tc_fence_before();
-  if constexpr (PAIR) cluster_sync(); else __syncthreads();
+  if constexpr (KIND != TILE_ONE) cluster_sync(); else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr_smem;
   grid_dependency_wait();
@@ -304,7 +400,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
         int tm, tn;
         tile_coords(tile, p, tm, tn);
         const int m0 = tm * L::BM + rank * 128, n0 = tn * BN + rank * L::B_ROWS;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
           if (elect_one()) {
             if constexpr (PAIR) {
@@ -332,7 +428,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       uint32_t phase = 0, slot_phase = 0;
       bool ok = true;
       for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
-        for (int kb = 0; kb < p.num_kb; ++kb) {
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
           // the data first: a slot is what comes late, and each wait costs about a hundred clocks
           if (!mbar_wait_spin(bar_full + s * 8, phase, abort_flag) || !mbar_wait_spin(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag)) {
             ok = false;
@@ -377,17 +473,17 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       tile_coords(tile, p, tm, tn);
       sa = p.sa + min(tm * L::BM + rank * 128 + q * 32 + lane, p.M - 1) * p.sa_m;
       sb = p.sb + min((tn * BN + h * HALF) / KB, p.nblocks - 1) * p.sb_n;
-      fa = *sa;
-      fb = *sb;
+      fa = sa[kb_begin * p.sa_k];
+      fb = sb[kb_begin * p.sb_k];
     };
     if (unit < num_tiles) first_scales(unit);
     for (int tile = unit; tile < num_tiles && ok; tile += num_units) {
       uint64_t acc[HALF / 2];
 #pragma unroll
       for (int j = 0; j < HALF / 2; ++j) acc[j] = 0;
-      for (int kb = 0; kb < p.num_kb; ++kb) {
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
         const uint64_t f = pack2(fa * fb, fa * fb);
-        if (kb + 1 < p.num_kb) {                     // the next block's scales arrive under this block's sums
+        if (kb + 1 < kb_end) {                       // the next block's scales arrive under this block's sums
           fa = sa[(kb + 1) * p.sa_k];
           fb = sb[(kb + 1) * p.sb_k];
         }
@@ -418,7 +514,49 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       tile_coords(tile, p, tm, tn);
       const int row0 = tm * L::BM + rank * 128 + q * 32, col0 = tn * BN + h * HALF;
       if (tile + num_units < num_tiles) first_scales(tile + num_units);   // arrive under this tile's output
-      if (ok) write_half<HALF>(p, &tmC, stage_mine, lane, row0, col0, acc);
+      if constexpr (SPLIT) {
+        // The CTAs add their sums up: a warp's columns go, sixteen at a time, to the CTA that writes them,
+        // into its ring -- which is free once its own last k-block is done (xready) -- and are added
+        // there in k order.  Warp w of a CTA deals with warps w alone.
+        static_assert(HALF == 64, "four pieces of sixteen columns");
+        constexpr int PIECE = 32 * 16 * 4;             // bytes of 32 rows x 16 columns
+        const int w = warp - EPI_WARP0, S = p.split;
+        auto first_piece = [&](int c) { return 4 * c / S; };
+        if (!ok) break;
+        if (lane < S) mbar_arrive_release_cluster(mapa(bar_xready + w * 8, lane));
+        ok = mbar_wait_acquire_cluster(bar_xready + w * 8, 0, abort_flag);
+        if (!ok) break;
+        int to = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          while (c >= first_piece(to + 1)) ++to;
+          const uint32_t dst = mapa(smem_base + (((c - first_piece(to)) * S + part) * EPI_WARPS + w) * PIECE + lane * 16, to);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 x = unpack2(acc[c * 8 + 2 * j]), y = unpack2(acc[c * 8 + 2 * j + 1]);
+            st_cluster_v4(dst + j * 512, make_float4(x.x, x.y, y.x, y.y));
+          }
+        }
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        __syncwarp();
+        if (lane < S) mbar_arrive_release_cluster(mapa(bar_xfull + w * 8, lane));
+        ok = mbar_wait_acquire_cluster(bar_xfull + w * 8, 0, abort_flag);
+        if (!ok) break;
+        for (int c = first_piece(part); c < first_piece(part + 1); ++c) {
+          float f[16] = {};
+          for (int from = 0; from < S; ++from) {
+            const uint8_t* src = smem + (((c - first_piece(part)) * S + from) * EPI_WARPS + w) * PIECE + lane * 16;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 v = *reinterpret_cast<const float4*>(src + j * 512);
+              f[4 * j] += v.x; f[4 * j + 1] += v.y; f[4 * j + 2] += v.z; f[4 * j + 3] += v.w;
+            }
+          }
+          put16<EPI>(p, row0 + lane, col0 + c * 16, f);
+        }
+      } else {
+        if (ok) write_half<EPI, HALF>(p, &tmC, stage_mine, lane, row0, col0, acc);
+      }
     }
     if (p.tma_store && lane == 0) tma_store_wait<0>();   // the staged blocks have left shared memory and landed
     if (!ok && lane == 0) report_timeout(p.status, 3);
@@ -428,24 +566,30 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
   // of a pair, neither CTA may leave while its partner can still signal its barriers or read its
   // shared memory
   tc_fence_before();
-  if constexpr (PAIR) cluster_sync(); else __syncthreads();
+  if constexpr (KIND != TILE_ONE) cluster_sync(); else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<GROUP>(tmem_base, L::TMEM_COLS);
   }
 }
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, int EPI>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
 hb_matmul_scaled_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                         const __grid_constant__ CUtensorMap tmC, const __grid_constant__ TileParams p) {
-  scaled_tile_body<false, BN, STAGES>(tmA, tmB, tmC, p);
+  scaled_tile_body<TILE_ONE, BN, STAGES, EPI>(tmA, tmB, tmC, p);
 }
-template <int BN, int STAGES>
+template <int BN, int STAGES, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TILE_THREADS, 1)
 hb_matmul_scaled_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                              const __grid_constant__ CUtensorMap tmC, const __grid_constant__ TileParams p) {
-  scaled_tile_body<true, BN, STAGES>(tmA, tmB, tmC, p);
+  scaled_tile_body<TILE_PAIR, BN, STAGES, EPI>(tmA, tmB, tmC, p);
+}
+template <int BN, int STAGES, int EPI>
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+hb_matmul_scaled_split_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                              const __grid_constant__ CUtensorMap tmC, const __grid_constant__ TileParams p) {
+  scaled_tile_body<TILE_SPLIT, BN, STAGES, EPI>(tmA, tmB, tmC, p);
 }
 
 hb_status make_maps(hb_ctx* ctx, const ScaledArgs& g, int b_rows, CUtensorMap* tmA, CUtensorMap* tmB, CUtensorMap* tmC, int* tma_store) {
@@ -469,12 +613,14 @@ hb_status make_maps(hb_ctx* ctx, const ScaledArgs& g, int b_rows, CUtensorMap* t
   return st;
 }
 
-template <bool PAIR, int BN, int STAGES>
-hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g) {
-  using L = TileLayout<PAIR, BN, STAGES>;
+template <int KIND, int BN, int STAGES, int EPI>
+hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
+  using L = TileLayout<KIND, BN, STAGES>;
+  constexpr bool PAIR = L::PAIR;
   void (*kern)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const TileParams);
-  if constexpr (PAIR) kern = hb_matmul_scaled_pair_kernel<BN, STAGES>;
-  else kern = hb_matmul_scaled_kernel<BN, STAGES>;
+  if constexpr (PAIR) kern = hb_matmul_scaled_pair_kernel<BN, STAGES, EPI>;
+  else if constexpr (KIND == TILE_SPLIT) kern = hb_matmul_scaled_split_kernel<BN, STAGES, EPI>;
+  else kern = hb_matmul_scaled_kernel<BN, STAGES, EPI>;
   // persistent CTAs (or pairs) that can run at once; of pairs the occupancy query knows, because not
   // every SM has a neighbour to pair with
   static int resident[64] = {};
@@ -510,11 +656,28 @@ hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g) {
   if (tiles_m * tiles_n > INT32_MAX / 2) return hb_fail(ctx, HB_ERR_UNSUPPORTED, "matmul_scaled: problem too large");
   p.tiles_m = (int)tiles_m; p.tiles_n = (int)tiles_n;
   p.raster_group = 8;
-  p.epilogue = g.epilogue;
   p.status = ctx->d_status;
   const int tiles = p.tiles_m * p.tiles_n, most = resident[ctx->device & 63];
-  const unsigned ctas = (PAIR ? 2 : 1) * (unsigned)(tiles < most ? tiles : most);
-  const cudaError_t e = hb_launch_dependent(kern, dim3(ctas), dim3(TILE_THREADS), L::DYN_BYTES, ctx->stream, tmA, tmB, tmC, p);
+  p.split = split;
+  cudaError_t e;
+  if constexpr (KIND == TILE_SPLIT) {              // one tile per cluster, not persistent: the ring ends as the exchange
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles * split);
+    cfg.blockDim = dim3(TILE_THREADS);
+    cfg.dynamicSmemBytes = L::DYN_BYTES;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, kern, tmA, tmB, tmC, p);
+  } else {
+    const unsigned ctas = (PAIR ? 2 : 1) * (unsigned)(tiles < most ? tiles : most);
+    e = hb_launch_dependent(kern, dim3(ctas), dim3(TILE_THREADS), L::DYN_BYTES, ctx->stream, tmA, tmB, tmC, p);
+  }
   if (e != cudaSuccess) { cudaGetLastError(); return hb_check_cuda(ctx, e, "matmul_scaled launch"); }
   ctx->launches++;
   return HB_OK;
@@ -571,28 +734,6 @@ struct FewLayout {
   static constexpr int DYN_BYTES = OFF_ABORT + 4 + 1024;
   static_assert(DYN_BYTES <= 227 * 1024 && STAGES >= 4, "ring does not fit shared memory");
 };
-
-// Arrive on / wait for a barrier when the data it stands for crossed between CTAs of the cluster.
-__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t bar_cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
-}
-__device__ __forceinline__ bool mbar_wait_acquire_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  for (uint32_t i = 0; i < HB_SPIN_LIMIT; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.b32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-    if ((i & 1023u) == 1023u && *abort_flag) return false;
-  }
-  *abort_flag = 1;
-  return false;
-}
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
 
 template <int MP>
 __global__ void __launch_bounds__(FEW_THREADS, 1)
@@ -945,22 +1086,44 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
   return HB_OK;
 }
 
+template <int KIND, int BN, int STAGES>
+hb_status launch_tile(hb_ctx* ctx, const ScaledArgs& g, int split = 1) {
+  switch (g.epilogue) {
+    case HB_EPI_GELU: return launch_tile_epi<KIND, BN, STAGES, HB_EPI_GELU>(ctx, g, split);
+    case HB_EPI_SWIGLU: return launch_tile_epi<KIND, BN, STAGES, HB_EPI_SWIGLU>(ctx, g, split);
+    case HB_EPI_RESIDUAL: return launch_tile_epi<KIND, BN, STAGES, HB_EPI_RESIDUAL>(ctx, g, split);
+    default: return launch_tile_epi<KIND, BN, STAGES, HB_EPI_NONE>(ctx, g, split);
+  }
+}
+
 hb_status launch(hb_ctx* ctx, const ScaledArgs& g) {
   if (g.M <= FEW_MAX_M)
     return g.M <= 16 ? launch_few<16>(ctx, g) : g.M <= 32 ? launch_few<32>(ctx, g) : launch_few<64>(ctx, g);
-  // The tile whose waves take the least time.  A k-block costs, with one wave on the GPU (K = 4096,
-  // microseconds): 0.47 for 256 x 256 on a CTA pair, 0.36 for 256 x 128 on a pair, 0.50 for 128 x 256 on one
-  // CTA.  Measured, in that order: 512 x 6144 19.4 / 23.0 / 20.2 us, 512 x 4096 18.3 / 13.8 / 19.3, 128 x
-  // 28672 34.3 / 41.5 / 25.8, 4096 x 4096 65 / 81 / 70.
-  const auto cost = [&](int64_t bm, int64_t bn, int64_t at_once, double kblock) {
+  // The form that takes the least time, in microseconds: a fixed part and a k-block's time per wave of
+  // tiles.  Measured (K = 4096; 256 x 256 pair, 256 x 128 pair, 128 x 256, split 2, split 4):
+  //   128 x 4096: 18.0 / 14.2 / 20.0 / 11.6 / 10.8      128 x 28672: 33.5 / 41.3 / 25.8 / 54 / 80
+  //   512 x 4096: 17.4 / 13.7 / 19.6 / 25.8 / 43.9      4096 x 4096: 65 / 81 / 70 / - / -
+  //   128 x 4096, K = 14336: 46.7 / 35.0 / 55.5 / 26.1 / 19.5
+  const double kblocks = (double)((g.K + KB - 1) / KB);
+  const auto waves = [&](int64_t bm, int64_t bn, int64_t at_once) {
     const int64_t tiles = (g.M + bm - 1) / bm * ((g.N + bn - 1) / bn);
-    return (double)((tiles + at_once - 1) / at_once) * kblock;
+    return (double)((tiles + at_once - 1) / at_once);
   };
-  const double pair_wide = cost(256, 256, ctx->sm_count / 2, 0.47), pair_narrow = cost(256, 128, ctx->sm_count / 2, 0.36),
-               one = cost(128, 256, ctx->sm_count, 0.50);
-  if (pair_wide <= pair_narrow && pair_wide <= one) return launch_tile<true, 256, 5>(ctx, g);
-  if (pair_narrow <= one) return launch_tile<true, 128, 6>(ctx, g);
-  return launch_tile<false, 256, 3>(ctx, g);
+  const double pair_wide = 5.5 + 0.42 * kblocks * waves(256, 256, ctx->sm_count / 2),
+               pair_narrow = 3.6 + 0.30 * kblocks * waves(256, 128, ctx->sm_count / 2),
+               one = 5.0 + 0.47 * kblocks * waves(128, 256, ctx->sm_count);
+  int split = 0;
+  double best = pair_wide < pair_narrow ? pair_wide : pair_narrow;
+  if (one < best) best = one;
+  for (int c = 2; c <= SPLIT_MAX && c <= kblocks; ++c) {
+    // clusters of c find room on most of the SMs only (148 SMs: 74, 45, 33)
+    const double t = 5.0 + 1.3 * c + 0.325 * ceil(kblocks / c) * waves(128, 128, ctx->sm_count * 9 / 10 / c);
+    if (t < best) { best = t; split = c; }
+  }
+  if (split) return launch_tile<TILE_SPLIT, 128, 4>(ctx, g, split);
+  if (best == pair_wide) return launch_tile<TILE_PAIR, 256, 5>(ctx, g);
+  if (best == pair_narrow) return launch_tile<TILE_PAIR, 128, 6>(ctx, g);
+  return launch_tile<TILE_ONE, 256, 3>(ctx, g);
 }
 
 hb_status decode(hb_ctx* ctx, const hb_tensor* A, const hb_tensor* sa, const hb_tensor* B, const hb_tensor* sb,

@@ -251,7 +251,9 @@ class COut:
 # rows around the limits of the few-row kernel and of the tiles; columns around blocks of 128; k around 128 and 16
 PRODUCTS = [(1, 256, 128), (1, 1, 1), (1, 6144, 512), (2, 300, 100), (16, 256, 4096), (16, 1000, 1000), (17, 384, 136), (63, 130, 300),
             (64, 512, 2048), (65, 512, 256), (64, 100, 128), (128, 128, 128), (129, 129, 129), (200, 255, 384), (256, 256, 640),
-            (300, 1000, 520), (333, 72, 2056), (511, 1025, 16), (700, 520, 1160), (1000, 8, 256), (1500, 2304, 384)]
+            (300, 1000, 520), (333, 72, 2056), (511, 1025, 16), (700, 520, 1160), (1000, 8, 256), (1500, 2304, 384),
+            # long sums of few tiles (split over a cluster), and a wide product of one tile row (128 x 256 tiles)
+            (65, 130, 7000), (128, 520, 4096), (200, 100, 6000), (100, 9500, 256), (128, 10000, 200)]
 
 
 @pytest.mark.parametrize("M,N,K", PRODUCTS)
@@ -272,7 +274,8 @@ def test_matmul_scaled(ctx, M, N, K):
 
 
 @pytest.mark.parametrize("epi", [hb.HB_EPI_GELU, hb.HB_EPI_SWIGLU, hb.HB_EPI_RESIDUAL])
-@pytest.mark.parametrize("M,N,K", [(1, 256, 128), (16, 512, 384), (64, 264, 1000), (129, 136, 200), (300, 1000, 520), (513, 770, 256)])
+@pytest.mark.parametrize("M,N,K", [(1, 256, 128), (16, 512, 384), (64, 264, 1000), (129, 136, 200), (300, 1000, 520), (513, 770, 256),
+                                   (100, 202, 6100), (128, 9600, 200), (1300, 2310, 136)])
 def test_matmul_scaled_epilogues(ctx, M, N, K, epi):
     rng = np.random.default_rng(M + N + K + epi)
     ab, sa, av = qr.operands(rng, M, K, 1)
@@ -306,7 +309,8 @@ def test_matmul_scaled_epilogues(ctx, M, N, K, epi):
         ctx.free(R)
 
 
-@pytest.mark.parametrize("M,N,K", [(16, 512, 1024), (48, 256, 512), (130, 300, 640), (600, 520, 896)])
+@pytest.mark.parametrize("M,N,K", [(16, 512, 1024), (48, 256, 512), (130, 300, 640), (600, 520, 896), (100, 300, 6400), (128, 9600, 384),
+                                   (1300, 2304, 384)])
 def test_matmul_scaled_is_exact_on_small_integers(ctx, M, N, K):
     """Integers up to 8 and power-of-two scales: every partial sum fits fp32, so the result is the
     exact sum rounded to bf16, whatever the order.  A scale that lands on the wrong row, column or
