@@ -58,8 +58,13 @@ namespace {
 
 const char* kNodeNames[] = {"matmul", "attention", "all_reduce", "rmsnorm", "rope", "embedding",
                             "swiglu", "gelu", "add", "argmax", "all_reduce_norm", "rope_append", "attention_decode",
-                            "advance"};
-size_t elem_size(int dtype) { return dtype == HB_BF16 ? 2 : 4; }
+                            "advance", "quantize", "rmsnorm_quant", "swiglu_quant", "matmul_scaled"};
+size_t elem_size(int dtype) { return dtype == HB_BF16 ? 2 : dtype == HB_E4M3 ? 1 : 4; }
+
+// Index of the input that a quantising node writes (the scales), -1 for every other node.
+int scale_slot(int kind) {
+  return kind == HB_NODE_QUANTIZE || kind == HB_NODE_SWIGLU_QUANT ? 1 : kind == HB_NODE_RMSNORM_QUANT ? 2 : -1;
+}
 
 int root_of(const hb_graph* g, int id) {
   while (g->tensors[id].kind == 2) id = g->tensors[id].base;
@@ -138,7 +143,7 @@ extern "C" hb_status hb_graph_temp(hb_graph* g, int32_t dtype, int32_t rank, con
                                    int32_t* id) {
   if (!g || !id || !shape) return HB_ERR_INVALID;
   if (rank < 1 || rank > 4) return hb_fail(g->ctx, HB_ERR_INVALID, "graph: rank must be 1..4");
-  if (dtype != HB_BF16 && dtype != HB_F32 && dtype != HB_I32) return hb_fail(g->ctx, HB_ERR_INVALID, "graph: dtype %d", dtype);
+  if (dtype != HB_BF16 && dtype != HB_F32 && dtype != HB_I32 && dtype != HB_E4M3) return hb_fail(g->ctx, HB_ERR_INVALID, "graph: dtype %d", dtype);
   hb_graph_tensor x;
   x.kind = 1;
   x.dtype = dtype;
@@ -196,8 +201,8 @@ extern "C" hb_status hb_graph_view(hb_graph* g, int32_t base, int64_t offset, in
 
 extern "C" hb_status hb_graph_add(hb_graph* g, const hb_node* n) {
   if (!g || !n) return HB_ERR_INVALID;
-  if (n->kind < 0 || n->kind > HB_NODE_ADVANCE) return hb_fail(g->ctx, HB_ERR_INVALID, "graph: unknown node kind %d", n->kind);
-  static const int n_in[] = {2, 3, 0, 2, 0, 2, 1, 1, 2, 1, 1, 2, 3, 0};   // required leading inputs per kind
+  if (n->kind < 0 || n->kind > HB_NODE_MATMUL_SCALED) return hb_fail(g->ctx, HB_ERR_INVALID, "graph: unknown node kind %d", n->kind);
+  static const int n_in[] = {2, 3, 0, 2, 0, 2, 1, 1, 2, 1, 1, 2, 3, 0, 2, 3, 2, 4};   // required leading inputs per kind
   for (int i = 0; i < 4; ++i) {
     if (i < n_in[n->kind] && !valid_id(g, n->in[i]))
       return hb_fail(g->ctx, HB_ERR_NOT_FOUND, "graph: %s node input %d names unknown tensor %d", kNodeNames[n->kind], i, n->in[i]);
@@ -205,6 +210,8 @@ extern "C" hb_status hb_graph_add(hb_graph* g, const hb_node* n) {
       return hb_fail(g->ctx, HB_ERR_NOT_FOUND, "graph: %s node optional input %d names unknown tensor %d", kNodeNames[n->kind], i, n->in[i]);
   }
   if (!valid_id(g, n->out)) return hb_fail(g->ctx, HB_ERR_NOT_FOUND, "graph: %s node output names unknown tensor %d", kNodeNames[n->kind], n->out);
+  if (n->kind == HB_NODE_MATMUL_SCALED && (n->iparam[0] & 0xff) == HB_EPI_RESIDUAL)
+    return hb_fail(g->ctx, HB_ERR_UNSUPPORTED, "graph: a matmul_scaled node has no residual input");
   // Only the collective nodes may run on the side stream.  The executor orders nodes on
   // different streams by the byte ranges of their tensors; compute nodes also share state it
   // cannot see (the stream-K workspace and tickets, the RoPE angle table, the attention work
@@ -276,13 +283,16 @@ extern "C" hb_status hb_graph_plan(hb_graph* g, size_t* arena_bytes, size_t* sym
     const hb_node& n = g->nodes[i];
     for (int k = 0; k < 4; ++k) {
       if (n.in[k] < 0) continue;
-      if (n.kind == HB_NODE_AR_NORM && k == 3) continue;   // residual_out is written, not read
+      if ((n.kind == HB_NODE_AR_NORM && k == 3) || k == scale_slot(n.kind)) continue;   // written, not read
       const int r = root_of(g, n.in[k]);
       if (g->tensors[r].kind != 1) continue;
       bool written = false;
-      for (int j = 0; j < i && !written; ++j)
+      for (int j = 0; j < i && !written; ++j) {
+        const int scale = scale_slot(g->nodes[j].kind);
         written = root_of(g, g->nodes[j].out) == r ||
-                  (g->nodes[j].kind == HB_NODE_AR_NORM && g->nodes[j].in[3] >= 0 && root_of(g, g->nodes[j].in[3]) == r);
+                  (g->nodes[j].kind == HB_NODE_AR_NORM && g->nodes[j].in[3] >= 0 && root_of(g, g->nodes[j].in[3]) == r) ||
+                  (scale >= 0 && root_of(g, g->nodes[j].in[scale]) == r);
+      }
       if (!written)
         return hb_fail(ctx, HB_ERR_INVALID, "graph: node %d (%s) reads planner-owned tensor %d before any node writes it", i,
                        kNodeNames[n.kind], n.in[k]);
@@ -364,7 +374,8 @@ extern "C" hb_status hb_graph_plan(hb_graph* g, size_t* arena_bytes, size_t* sym
       for (int k = 0; k < 4; ++k)
         if (n.in[k] >= 0)
           foot[i].push_back(range_of(n.in[k], (n.kind == HB_NODE_RMSNORM && k == 2) || (n.kind == HB_NODE_AR_NORM && k == 3) ||
-                                                  (n.kind == HB_NODE_ATTENTION && k == 3) || (n.kind == HB_NODE_ROPE_APPEND && k == 0)));   // inputs the node writes
+                                                  (n.kind == HB_NODE_ATTENTION && k == 3) || (n.kind == HB_NODE_ROPE_APPEND && k == 0) ||
+                                                  k == scale_slot(n.kind) || (n.kind == HB_NODE_RMSNORM_QUANT && k == 3)));   // inputs the node writes
       foot[i].push_back(range_of(n.out, true));
     }
     g->wait_for.assign(nn, -1);
@@ -517,6 +528,34 @@ static hb_status run_node(hb_graph* g, int i) {
         if (T(n.out).dtype != HB_I32) { st = hb_fail(ctx, HB_ERR_INVALID, "graph: advance needs an i32 position"); break; }
         st = hb_advance_pos(ctx, static_cast<int32_t*>(T(n.out).ptr), n.iparam[0]);
         break;
+      case HB_NODE_QUANTIZE: {
+        hb_tensor x = as_tensor(T(n.in[0])), s = as_tensor(T(n.in[1])), q = as_tensor(T(n.out));
+        st = hb_quantize(ctx, &x, &q, &s, n.iparam[0]);
+        break;
+      }
+      case HB_NODE_RMSNORM_QUANT: {
+        hb_tensor x = as_tensor(T(n.in[0])), s = as_tensor(T(n.in[2])), q = as_tensor(T(n.out)), r;
+        if (n.in[3] >= 0) r = as_tensor(T(n.in[3]));
+        const hb_graph_tensor& gain = T(n.in[1]);
+        if (gain.dtype != HB_BF16 || !is_contiguous(gain) || x.rank != 2 || numel(gain) != x.shape[1]) {
+          st = hb_fail(ctx, HB_ERR_INVALID, "graph: rmsnorm_quant needs a contiguous bf16 gain of one value per column");
+          break;
+        }
+        st = hb_rmsnorm_quant(ctx, &x, T(n.in[1]).ptr, &q, &s, n.in[3] >= 0 ? &r : nullptr, n.fparam[0]);
+        break;
+      }
+      case HB_NODE_SWIGLU_QUANT: {
+        hb_tensor x = as_tensor(T(n.in[0])), s = as_tensor(T(n.in[1])), q = as_tensor(T(n.out));
+        st = hb_swiglu_quant(ctx, &x, &q, &s);
+        break;
+      }
+      case HB_NODE_MATMUL_SCALED: {
+        hb_tensor a = as_tensor(T(n.in[0])), sa = as_tensor(T(n.in[1])), b = as_tensor(T(n.in[2])), sb = as_tensor(T(n.in[3])),
+                  c = as_tensor(T(n.out));
+        hb_matmul_opts o = {n.iparam[0], -1, nullptr, 0};
+        st = hb_matmul_scaled(ctx, &a, &sa, &b, &sb, &c, &o);
+        break;
+      }
       case HB_NODE_ARGMAX: {
         const hb_graph_tensor& x = T(n.in[0]);
         st = hb_argmax(ctx, x.ptr, static_cast<int32_t*>(T(n.out).ptr), x.shape[0], x.shape[1]);
@@ -650,7 +689,7 @@ extern "C" hb_status hb_graph_describe(hb_graph* g, char* buf, size_t len) {
   for (int i = 0; i < (int)g->tensors.size(); ++i) {
     const hb_graph_tensor& t = g->tensors[i];
     if (t.kind != 1) continue;
-    snprintf(line, sizeof(line), "t%d %s bytes %zu live [%d,%d] %s+%zu\n", i, t.dtype == HB_BF16 ? "bf16" : t.dtype == HB_F32 ? "f32" : "i32",
+    snprintf(line, sizeof(line), "t%d %s bytes %zu live [%d,%d] %s+%zu\n", i, t.dtype == HB_BF16 ? "bf16" : t.dtype == HB_F32 ? "f32" : t.dtype == HB_E4M3 ? "e4m3" : "i32",
              t.bytes, t.first, t.last, t.in_symmetric ? "sym" : "arena", t.arena_off);
     s += line;
   }

@@ -9,7 +9,8 @@ from . import _capi
 from .model_ir import Context, Tensor, _contig, _lib
 
 (NODE_MATMUL, NODE_ATTENTION, NODE_ALL_REDUCE, NODE_RMSNORM, NODE_ROPE, NODE_EMBEDDING, NODE_SWIGLU, NODE_GELU,
- NODE_ADD, NODE_ARGMAX, NODE_AR_NORM, NODE_ROPE_APPEND, NODE_ATTN_DECODE, NODE_ADVANCE) = range(14)
+ NODE_ADD, NODE_ARGMAX, NODE_AR_NORM, NODE_ROPE_APPEND, NODE_ATTN_DECODE, NODE_ADVANCE, NODE_QUANTIZE,
+ NODE_RMSNORM_QUANT, NODE_SWIGLU_QUANT, NODE_MATMUL_SCALED) = range(18)
 T_SYMMETRIC = 1
 
 
@@ -104,6 +105,24 @@ class Graph:
 
     def advance(self, pos, n=1):
         return self._add(NODE_ADVANCE, [], pos, [n])
+
+    def temp_quantised(self, rows: int, cols: int):
+        """Planner-owned (q, scale) of a row-quantised [rows, cols]; cols a multiple of 16."""
+        return self.temp((rows, cols), _capi.HB_E4M3), self.temp((rows, (cols + 127) // 128), _capi.HB_F32)
+
+    def quantize(self, x, out, scale, block_rows=1):
+        return self._add(NODE_QUANTIZE, [x, scale], out, [block_rows])
+
+    def rmsnorm_quant(self, x, gain, out, scale, residual=None, eps=1e-5):
+        return self._add(NODE_RMSNORM_QUANT, [x, gain, scale, residual], out, [], [eps])
+
+    def swiglu_quant(self, x, out, scale):
+        return self._add(NODE_SWIGLU_QUANT, [x, scale], out)
+
+    def matmul_scaled(self, a, a_scale, b, b_scale, out, epilogue=_capi.HB_EPI_NONE, weights=False):
+        """`a`, `b`: quantised operands with their scales (``Context.matmul_scaled``)."""
+        return self._add(NODE_MATMUL_SCALED, [a, a_scale, b, b_scale], out,
+                         [epilogue | (_capi.HB_MATMUL_WEIGHTS_B if weights else 0)])
 
     def embedding(self, table, ids, out):
         return self._add(NODE_EMBEDDING, [table, ids], out)

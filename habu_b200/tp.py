@@ -84,6 +84,69 @@ def shard_layer(full: Dict[str, np.ndarray], cfg: DecoderConfig, world: int, ran
             "wgu": wgu, "wd": np.ascontiguousarray(full["wd"][:, f0:f1]), "g1": full["g1"], "g2": full["g2"]}
 
 
+QUANTISED = ("wqkv", "wo", "wgu", "wd")       # the weight matrices of a layer; the gains stay bf16
+
+
+def upload_layer(ctx, layer: Dict[str, np.ndarray], e4m3: bool) -> Dict[str, object]:
+    """Device tensors of one layer's weights (bf16 bit patterns).  With `e4m3` every matrix is
+    quantised on the device in 128 x 128 blocks (a (q, scale) pair instead of a tensor) and its
+    bf16 copy is freed."""
+    dev = {}
+    for k, v in layer.items():
+        t = ctx.upload(v)
+        if e4m3 and k in QUANTISED:
+            dev[k] = ctx.quantize(t, block_rows=128)
+            ctx.sync()
+            ctx.free(t)
+        else:
+            dev[k] = t
+    return dev
+
+
+class _Products:
+    """The products of a layer on an executor graph, in bf16 or with e4m3 operands: where an activation
+    comes from (a norm, SwiGLU, attention) and the product that takes it."""
+
+    def __init__(self, g, e4m3: bool, eps: float, weights: bool):
+        self.g, self.e4m3, self.eps, self.weights = g, e4m3, eps, weights
+
+    def weight(self, v):
+        """Graph ids of one weight: B as [in, out], and its scales."""
+        return (self.g.input(v[0].T), self.g.input(v[1].T)) if isinstance(v, tuple) else self.g.input(v.T)
+
+    def norm(self, x, gain, rows, cols, residual=None):
+        if self.e4m3:
+            h = self.g.temp_quantised(rows, cols)
+            self.g.rmsnorm_quant(x, gain, *h, residual=residual, eps=self.eps)
+        else:
+            h = self.g.temp((rows, cols))
+            self.g.rmsnorm(x, gain, h, residual=residual, eps=self.eps)
+        return h
+
+    def swiglu(self, gu, rows, half):
+        if self.e4m3:
+            act = self.g.temp_quantised(rows, half)
+            self.g.swiglu_quant(gu, *act)
+        else:
+            act = self.g.temp((rows, half))
+            self.g.swiglu(gu, act)
+        return act
+
+    def operand(self, x, rows, cols):
+        """A bf16 activation as an operand of :meth:`matmul`."""
+        if not self.e4m3:
+            return x
+        h = self.g.temp_quantised(rows, cols)
+        self.g.quantize(x, *h)
+        return h
+
+    def matmul(self, a, w, out, epilogue=_capi.HB_EPI_NONE):
+        if self.e4m3:
+            self.g.matmul_scaled(*a, *w, out, epilogue=epilogue, weights=self.weights)
+        else:
+            self.g.matmul(a, w, out, epilogue=epilogue, weights=self.weights)
+
+
 class DecoderGraph:
     """Node list of the decoder forward for one rank; weights are bf16 bit patterns.
 
@@ -95,12 +158,18 @@ class DecoderGraph:
 
     def __init__(self, ctx, cfg: DecoderConfig, world: int, rank: int, layers: List[Dict[str, np.ndarray]],
                  algo: int = _capi.HB_AR_AUTO, chunks: int = 1, fused: bool = False, gathered: bool = False,
-                 fused_form: int = 0, fused_ctas: int = 0, share=None):
-        """`fused_form` / `fused_ctas`: kernel form of the fused collective for this graph's runs
+                 fused_form: int = 0, fused_ctas: int = 0, share=None, e4m3: bool = False):
+        """`e4m3`: weights and the inputs of their products in 8 bits (``Context.matmul_scaled``), one rank
+        only; attention, the residual stream and the outputs of the products stay bf16.  `fused_form` / `fused_ctas`: kernel form of the fused collective for this graph's runs
         (``Context.comm_configure``).  `share`: another DecoderGraph of the same rank whose uploaded
         weights and input buffer this one reuses (schedule variants of one model)."""
         from .graph import Graph
         check_shardable(cfg, world)
+        if e4m3 and world > 1:
+            raise ValueError("e4m3 weights are supported on one rank")
+        if share is not None and bool(e4m3) != share.e4m3:
+            raise ValueError("a graph shares weights only with one of the same precision")
+        self.e4m3 = bool(e4m3)
         self._out_id = None
         self.fused_form, self.fused_ctas, self._share = fused_form, fused_ctas, share
         self.schedule = {"chunks": chunks, "fused": bool(fused and world > 1), "gathered": bool(gathered and world > 1),
@@ -125,25 +194,25 @@ class DecoderGraph:
         x0, out = g.input(self.x0), g.input(self._out)
         rows = lambda t, c: g.view(t, c * Tc * d, (Tc, d), (d, 1))       # chunk c of a [T, d] tensor
         self.weights = []
+        ops = _Products(g, e4m3, cfg.eps, weights=False)
         x = None                                  # residual stream [T, d], planner-owned after layer 0
         pending = [None] * chunks                 # per chunk: sublayer output not yet added into the stream
         for li, lw in enumerate(layers):
-            dev = share.weights[li] if share is not None else {k: ctx.upload(v) for k, v in lw.items()}
+            dev = share.weights[li] if share is not None else upload_layer(ctx, lw, e4m3)
             self.weights.append(dev)
-            w = {k: g.input(v if k in ("g1", "g2") else v.T) for k, v in dev.items()}
+            w = {k: g.input(v) if k in ("g1", "g2") else ops.weight(v) for k, v in dev.items()}
             first = x is None
             if first:
                 x = g.temp((T, d))
             # ---- attention sublayer, chunk by chunk
             aos = []
             for c in range(chunks):
-                h = g.temp((Tc, d))
                 if first:
-                    g.rmsnorm(rows(x0, c), w["g1"], h, eps=cfg.eps)
+                    h = ops.norm(rows(x0, c), w["g1"], Tc, d)
                 else:
-                    g.rmsnorm(pending[c], w["g1"], h, residual=rows(x, c), eps=cfg.eps)
+                    h = ops.norm(pending[c], w["g1"], Tc, d, residual=rows(x, c))
                 qkv = g.temp((Tc, W))
-                g.matmul(h, w["wqkv"], qkv)
+                ops.matmul(h, w["wqkv"], qkv)
                 g.rope(g.view(qkv, 0, (Tc, ql * hd), (W, 1)), cfg.seq, ql, hd, cfg.rope_base)
                 g.rope(g.view(qkv, ql * hd, (Tc, kl * hd), (W, 1)), cfg.seq, kl, hd, cfg.rope_base)
                 v4 = lambda off, H: g.view(qkv, off, (Bc, cfg.seq, H, hd), (cfg.seq * W, W, hd, 1))
@@ -151,21 +220,20 @@ class DecoderGraph:
                 g.attention(v4(0, ql), v4(ql * hd, kl), v4((ql + kl) * hd, kl),
                             g.view(attn, 0, (Bc, cfg.seq, ql, hd), (cfg.seq * ql * hd, ql * hd, hd, 1)), causal=True)
                 ao = g.temp((Tc, d), symmetric=True)
-                g.matmul(attn, w["wo"], ao)
+                ops.matmul(ops.operand(attn, Tc, ql * hd), w["wo"], ao)
                 g.all_reduce(ao, algo, stream=side)
                 aos.append(ao)
             # ---- FFN sublayer, chunk by chunk
             for c in range(chunks):
-                h2 = g.temp((Tc, d))
                 if first:
                     g.add(rows(x0, c), aos[c], rows(x, c))
-                    g.rmsnorm(rows(x, c), w["g2"], h2, eps=cfg.eps)
+                    h2 = ops.norm(rows(x, c), w["g2"], Tc, d)
                 else:
-                    g.rmsnorm(aos[c], w["g2"], h2, residual=rows(x, c), eps=cfg.eps)
+                    h2 = ops.norm(aos[c], w["g2"], Tc, d, residual=rows(x, c))
                 act = g.temp((Tc, fl))
-                g.matmul(h2, w["wgu"], act, epilogue=_capi.HB_EPI_SWIGLU)
+                ops.matmul(h2, w["wgu"], act, epilogue=_capi.HB_EPI_SWIGLU)
                 fo = g.temp((Tc, d), symmetric=True)
-                g.matmul(act, w["wd"], fo)
+                ops.matmul(ops.operand(act, Tc, fl), w["wd"], fo)
                 g.all_reduce(fo, algo, stream=side)
                 pending[c] = fo
         for c in range(chunks):
@@ -332,9 +400,11 @@ class DecodeGraph:
     position fixed: the benchmark's steady-state step)."""
 
     def __init__(self, ctx, cfg: DecoderConfig, layers: List[Dict[str, np.ndarray]], batch: int, s_max: int,
-                 advance: bool = True, len_hint: int = 0):
+                 advance: bool = True, len_hint: int = 0, e4m3: bool = False):
+        """`e4m3`: weights and the inputs of their products in 8 bits (``Context.matmul_scaled``), which
+        halves the weight bytes of a step; the caches, attention and the residual stream stay bf16."""
         from .graph import Graph
-        self.ctx, self.cfg, self.batch, self.s_max = ctx, cfg, batch, s_max
+        self.ctx, self.cfg, self.batch, self.s_max, self.e4m3 = ctx, cfg, batch, s_max, bool(e4m3)
         d, hd, Hq, Hkv, F = cfg.d_model, cfg.head_dim, cfg.n_q_heads, cfg.n_kv_heads, cfg.ffn_hidden
         W = (Hq + 2 * Hkv) * hd
         B = batch
@@ -344,36 +414,34 @@ class DecodeGraph:
         self.pos = ctx.upload(np.zeros(1, np.int32))
         self.kv = [ctx.empty((2 * B, s_max, Hkv, hd)) for _ in layers]
         x_in, out, pos = g.input(self.x), g.input(self.out), g.input(self.pos)
-        self.weights = [{k: ctx.upload(v) for k, v in lw.items()} for lw in layers]
-        ws = [{k: g.input(v if k in ("g1", "g2") else v.T) for k, v in dev.items()} for dev in self.weights]
+        self.weights = [upload_layer(ctx, lw, e4m3) for lw in layers]
+        ops = _Products(g, e4m3, cfg.eps, weights=True)
+        ws = [{k: g.input(v) if k in ("g1", "g2") else ops.weight(v) for k, v in dev.items()} for dev in self.weights]
         xres = g.temp((B, d))                 # residual stream
         pending = None                        # sublayer output not yet added into the stream
         for li, w in enumerate(ws):
             kv = g.input(self.kv[li])
-            h = g.temp((B, d))
             if li == 0:
-                g.rmsnorm(x_in, w["g1"], h, eps=cfg.eps)
+                h = ops.norm(x_in, w["g1"], B, d)
             else:
-                g.rmsnorm(pending, w["g1"], h, residual=xres, eps=cfg.eps)
+                h = ops.norm(pending, w["g1"], B, d, residual=xres)
             qkv = g.temp((B, W))
-            g.matmul(h, w["wqkv"], qkv, weights=True)
+            ops.matmul(h, w["wqkv"], qkv)
             g.rope_append(qkv, pos, kv, Hq, Hkv, cfg.rope_base)
             attn = g.temp((B, Hq * hd))
             g.attention_decode(qkv, kv, pos, attn, Hq, Hkv, len_hint=len_hint)
             ao = g.temp((B, d))
-            g.matmul(attn, w["wo"], ao, weights=True)
-            h2 = g.temp((B, d))
+            ops.matmul(ops.operand(attn, B, Hq * hd), w["wo"], ao)
             if li == 0:
                 g.add(x_in, ao, xres)
-                g.rmsnorm(xres, w["g2"], h2, eps=cfg.eps)
+                h2 = ops.norm(xres, w["g2"], B, d)
             else:
-                g.rmsnorm(ao, w["g2"], h2, residual=xres, eps=cfg.eps)
+                h2 = ops.norm(ao, w["g2"], B, d, residual=xres)
             gu = g.temp((B, 2 * F))
-            g.matmul(h2, w["wgu"], gu, weights=True)
-            act = g.temp((B, F))
-            g.swiglu(gu, act)
+            ops.matmul(h2, w["wgu"], gu)
+            act = ops.swiglu(gu, B, F)
             fo = g.temp((B, d))
-            g.matmul(act, w["wd"], fo, weights=True)
+            ops.matmul(act, w["wd"], fo)
             pending = fo
         g.add(xres, pending, out)
         if advance:
@@ -406,6 +474,6 @@ class DecodeGraph:
         """Algorithmic HBM bytes of one step at cache length `length`: every weight once, the
         cached keys and values of every layer once."""
         cfg = self.cfg
-        w = sum(t.nbytes for dev in self.weights for k, t in dev.items())
+        w = sum(t.nbytes for dev in self.weights for v in dev.values() for t in (v if isinstance(v, tuple) else (v,)))
         kvb = len(self.kv) * 2.0 * self.batch * length * cfg.n_kv_heads * cfg.head_dim * 2
         return w + kvb

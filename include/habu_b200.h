@@ -343,7 +343,12 @@ enum {
                                 [2*batch, s_max, kv_heads, 128]   iparam: q heads, kv heads   fparam: base */
   HB_NODE_ATTN_DECODE = 12,  /* in: qkv, kv cache, pos; out: [batch, q_heads*128]
                                 iparam: q heads, kv heads, len_hint   fparam: scale */
-  HB_NODE_ADVANCE = 13       /* in place on `out` (i32[1])   iparam: increment */
+  HB_NODE_ADVANCE = 13,      /* in place on `out` (i32[1])   iparam: increment */
+  HB_NODE_QUANTIZE = 14,     /* in: x, scale (written); out: e4m3   iparam: block_rows */
+  HB_NODE_RMSNORM_QUANT = 15,  /* in: x, gain, scale (written), [residual]; out: e4m3   fparam: eps */
+  HB_NODE_SWIGLU_QUANT = 16, /* in: x, scale (written); out: e4m3 */
+  HB_NODE_MATMUL_SCALED = 17 /* in: A, a_scale, B, b_scale; out: C   iparam: epilogue (not HB_EPI_RESIDUAL: a node
+                                has four inputs; the norm or add behind it adds the residual) */
 };
 enum { HB_T_SYMMETRIC = 1 };
 typedef struct hb_node {
