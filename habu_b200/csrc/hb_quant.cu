@@ -7,7 +7,7 @@
 //
 // The floor keeps the scale normal and its reciprocal finite, so that a group of zeros (or of
 // values so small that 1 / scale would overflow) needs no case of its own.  y / scale is formed as
-// y * (1 / scale): 2^-23 off at most, against the 2^-4 of the rounding to e4m3 that follows.
+// y * (1 / scale): 2^-22 off at most, against the 2^-4 of the rounding to e4m3 that follows.
 // fmaxf drops NaNs, so a NaN does not spread over its group: its own product is NaN and converts
 // to the e4m3 NaN.
 #include <cuda_fp8.h>
@@ -32,10 +32,21 @@ __device__ __forceinline__ uint32_t f2_to_bf2(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// Two fp32 products, and two multiply-adds, in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\tmul.rn.f32x2 %0, x, y;\n\t}" : "=l"(d) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t d;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\tmov.b64 z, {%5, %6};\n\tfma.rn.f32x2 %0, x, y, z;\n\t}"
+      : "=l"(d) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
+  return r;
 }
 // Maximum over the 16 lanes that hold a group (8 values each); every lane of the warp takes part.
 __device__ __forceinline__ float group_max(float v) {
@@ -43,12 +54,19 @@ __device__ __forceinline__ float group_max(float v) {
   for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax / Q_TOP, Q_FLOOR); }
+// One multiplication by fl(1 / 448) (2^-23 off at most) and an approximate reciprocal (1 ulp): a division
+// each would be a fifth of the instructions of these kernels.
+__device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * (1.0f / Q_TOP), Q_FLOOR); }
+__device__ __forceinline__ float inverse_of(float scale) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  return r;
+}
 
 __device__ __forceinline__ float abs_max8(const float (&y)[8]) {
-  float m = fabsf(y[0]);
+  float m = 0.f;                                // NaNs drop out, eight of them too
 #pragma unroll
-  for (int k = 1; k < 8; ++k) m = fmaxf(m, fabsf(y[k]));
+  for (int k = 0; k < 8; k += 2) asm("max.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(fabsf(y[k])), "f"(fabsf(y[k + 1])));
   return m;
 }
 // Eight values to eight e4m3 bytes (to nearest even; beyond 448 saturates, NaN stays NaN).
@@ -56,18 +74,23 @@ __device__ __forceinline__ uint2 pack8(const float (&y)[8], float inv) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h] * inv, y[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[4 * h + 2] * inv, y[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+    const float2 k = make_float2(inv, inv);
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(mul2(make_float2(y[4 * h], y[4 * h + 1]), k), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(mul2(make_float2(y[4 * h + 2], y[4 * h + 3]), k), __NV_SATFINITE, __NV_E4M3);
     w[h] = lo | hi << 16;
   }
   return make_uint2(w[0], w[1]);
 }
 
 // ------------------------------------------------------------------ RMSNorm
-// One CTA per row, the row in registers, as in hb_rmsnorm: VEC 16-byte vectors per thread.
-// Sixteen neighbouring threads hold the 128 values of a group, so its maximum is four shuffles.
-constexpr int RMS_THREADS = 256;
-constexpr int RMS_MAX_VEC = 8;
+// `tpr` threads take a row (a power of two from 16 on), each VEC 16-byte vectors of it at fixed columns;
+// a CTA takes blockDim / tpr rows at a time and goes on to the next ones: it is persistent, so that the
+// next rows are on their way while the statistics of these are formed, and the gain is read once.
+// With h = x * gain, y = h * r and max|y| = max|h| * r for the row's r = rsqrt(..): the maxima of the groups
+// (sixteen neighbouring threads hold one: four shuffles) do not wait for the statistic.
+// Measured: 8192 x 4096 with the residual 37.6 us (6.2 TB/s, 95 % of a copy), without it 25.6 us (bound by
+// the instructions: 3.9 TB/s), 16 x 4096 2.2 us.  One CTA per row without the prefetch: 42.1 and 30.1 us.
+constexpr int RMS_MAX_COLS = 16384;
 
 struct NormParams {
   const __nv_bfloat16* x;
@@ -75,71 +98,99 @@ struct NormParams {
   __nv_bfloat16* residual;     // or null
   uint8_t* q;
   float* scale;
+  int64_t rows;
   int64_t ldx, ldr, ldq, ss0, ss1;
-  int cols8;
+  int cols8, tpr;
   float inv_cols, eps;
 };
 
-template <int VEC>
-__global__ void __launch_bounds__(RMS_THREADS) rmsnorm_quant_kernel(const NormParams p) {
-  __shared__ float red[RMS_THREADS / 32];
+template <int VEC, bool RES, int THREADS>
+__global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams p) {
+  __shared__ float red[2][THREADS / 32];
+  const int tpr = p.tpr, warps = tpr > 32 ? tpr / 32 : 1;           // warps that share a row
+  const int t = threadIdx.x & (tpr - 1);                            // thread of the row
+  const int sub_row = threadIdx.x / tpr, per_step = THREADS / tpr;
+  const int first_warp = sub_row * warps;                           // (tpr >= 32)
   HB_LAUNCH_DEPENDENTS();
-  const int64_t row = blockIdx.x;
-  const uint4* xr = reinterpret_cast<const uint4*>(p.x + row * p.ldx);
-  uint4* rr = p.residual ? reinterpret_cast<uint4*>(p.residual + row * p.ldr) : nullptr;
-  float v[VEC][8];
-  float ss = 0.f;
+  float2 gain[VEC][4];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const int c = threadIdx.x + i * RMS_THREADS;
+    const uint4 g = __ldg(p.gain + min(t + i * tpr, p.cols8 - 1));
+    const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
-    if (c < p.cols8) {
-      const uint4 a = xr[c];
-      const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
-      uint32_t rw[4] = {0, 0, 0, 0};
-      if (rr) { const uint4 r = rr[c]; rw[0] = r.x; rw[1] = r.y; rw[2] = r.z; rw[3] = r.w; }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float2 f = bf2_to_f2(aw[k]);
-        if (rr) {
-          const float2 g = bf2_to_f2(rw[k]);
-          // the updated residual is what gets normalised, after its own bf16 rounding
-          rw[k] = f2_to_bf2(f.x + g.x, f.y + g.y);
-          f = bf2_to_f2(rw[k]);
-        }
-        v[i][2 * k] = f.x;
-        v[i][2 * k + 1] = f.y;
-        ss += f.x * f.x + f.y * f.y;
-      }
-      if (rr) rr[c] = make_uint4(rw[0], rw[1], rw[2], rw[3]);
-    }
+    for (int k = 0; k < 4; ++k) gain[i][k] = bf2_to_f2(gw[k]);
   }
-  ss = warp_sum(ss);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  float tot = 0.f;
+  uint4 xn[VEC], rn[VEC];
+  auto fetch = [&](int64_t row) {                                   // past the edge: the last row and column again
+    const int64_t at = min(row, p.rows - 1);
 #pragma unroll
-  for (int w = 0; w < RMS_THREADS / 32; ++w) tot += red[w];
-  const float inv_rms = rsqrtf(tot * p.inv_cols + p.eps);
-  uint8_t* qr = p.q + row * p.ldq;
+    for (int i = 0; i < VEC; ++i) {
+      const int c = min(t + i * tpr, p.cols8 - 1);
+      xn[i] = *(reinterpret_cast<const uint4*>(p.x + at * p.ldx) + c);
+      if (RES) rn[i] = *(reinterpret_cast<const uint4*>(p.residual + at * p.ldr) + c);
+    }
+  };
+  int64_t row = static_cast<int64_t>(blockIdx.x) * per_step + sub_row;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per_step;
+  fetch(row);
+  int buf = 0;
+  for (; row - sub_row < p.rows; row += step, buf ^= 1) {           // every thread of the CTA takes every step
+    float h[VEC][8], top[VEC], ss = 0.f;                            // value * gain, and its maximum in the group
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const int c = threadIdx.x + i * RMS_THREADS;
-    if (c < p.cols8) {
-      const uint4 g = __ldg(p.gain + c);
-      const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+    for (int i = 0; i < VEC; ++i) {
+      const int c = t + i * tpr;
+      uint32_t w[4] = {xn[i].x, xn[i].y, xn[i].z, xn[i].w};
+      const uint32_t r[4] = {rn[i].x, rn[i].y, rn[i].z, rn[i].w};
+      float2 part = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 gf = bf2_to_f2(gw[k]);
-        v[i][2 * k] *= inv_rms * gf.x;
-        v[i][2 * k + 1] *= inv_rms * gf.y;
+        float2 f = bf2_to_f2(w[k]);
+        if (RES) {
+          // the updated residual is what gets normalised, after its own bf16 rounding
+          const float2 g = bf2_to_f2(r[k]);
+          w[k] = f2_to_bf2(f.x + g.x, f.y + g.y);
+          f = bf2_to_f2(w[k]);
+        }
+        part = fma2(f, f, part);
+        const float2 y = mul2(f, gain[i][k]);
+        h[i][2 * k] = y.x;
+        h[i][2 * k + 1] = y.y;
       }
+      const bool in = c < p.cols8;
+      if (in) ss += part.x + part.y;
+      if (RES && in && row < p.rows) *(reinterpret_cast<uint4*>(p.residual + row * p.ldr) + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      top[i] = in ? abs_max8(h[i]) : 0.f;
     }
-    const float s = scale_of(group_max(abs_max8(v[i])));
-    if (c < p.cols8) {
-      *reinterpret_cast<uint2*>(qr + c * 8) = pack8(v[i], 1.0f / s);
-      if ((threadIdx.x & 15) == 0) p.scale[row * p.ss0 + (c >> 4) * p.ss1] = s;
+    fetch(row + step);
+    for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (warps > 1 && (threadIdx.x & 31) == 0) red[buf][threadIdx.x >> 5] = ss;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) top[i] = group_max(top[i]);
+    if (warps > 1) {
+      __syncthreads();                                              // the other buffer is rewritten behind the next one
+      ss = 0.f;
+      for (int w = 0; w < warps; ++w) ss += red[buf][first_warp + w];
+    }
+    const float inv_rms = rsqrtf(ss * p.inv_cols + p.eps);
+    if (row < p.rows) {
+      uint8_t* qr = p.q + row * p.ldq;
+      float* sr = p.scale + row * p.ss0;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int c = t + i * tpr;
+        if (c < p.cols8) {
+          const float s = scale_of(top[i] * inv_rms);
+          // (two products: r / scale on its own would overflow for a group of zeros)
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) {
+            const float2 y = mul2(make_float2(h[i][k], h[i][k + 1]), make_float2(inv_rms, inv_rms));
+            h[i][k] = y.x;
+            h[i][k + 1] = y.y;
+          }
+          *reinterpret_cast<uint2*>(qr + c * 8) = pack8(h[i], inverse_of(s));
+          if ((c & 15) == 0) sr[(c >> 4) * p.ss1] = s;
+        }
+      }
     }
   }
 }
@@ -164,45 +215,64 @@ __device__ __forceinline__ float silu_f(float v) { return __fdividef(v, 1.0f + _
 // in whole 16-byte vectors.  Otherwise (odd widths, pitches or addresses) columns 16 apart inside the
 // same group of 128, so that neighbouring threads still read neighbouring elements.
 __device__ __forceinline__ int loose_col(int c, int k) { return (c >> 4) * QG + (c & 15) + 16 * k; }
+// load() only requests; widen() is where the thread first waits.  Rows and columns past the edge
+// repeat the last ones, so that no load hides behind a branch; the caller drops what it does not own.
 template <int SRC, bool VEC>
-__device__ __forceinline__ void load8(const RowParams& p, int64_t row, int c, float (&y)[8]) {
-  if constexpr (SRC == SRC_SWIGLU) {
-    const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.x) + row * p.ldx + c * 8;
-    const uint4 g = *reinterpret_cast<const uint4*>(base), u = *reinterpret_cast<const uint4*>(base + p.cols);
-    const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
+struct Values {
+  uint4 a, b;                  // VEC: the 16-byte vectors (b: the up half, or the second four fp32 values)
+  float f[8];                  // otherwise
+  __device__ __forceinline__ void load(const RowParams& p, int64_t row, int c) {
+    if constexpr (SRC == SRC_SWIGLU) {
+      const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.x) + row * p.ldx + c * 8;
+      a = *reinterpret_cast<const uint4*>(base);
+      b = *reinterpret_cast<const uint4*>(base + p.cols);
+    } else if constexpr (SRC == SRC_BF16) {
+      const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.x) + row * p.ldx;
+      if constexpr (VEC) {
+        a = *reinterpret_cast<const uint4*>(base + c * 8);
+      } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 a = bf2_to_f2(gw[k]), b = bf2_to_f2(uw[k]);
-      y[2 * k] = silu_f(a.x) * b.x;
-      y[2 * k + 1] = silu_f(a.y) * b.y;
-    }
-  } else if constexpr (SRC == SRC_BF16) {
-    const __nv_bfloat16* row_ptr = static_cast<const __nv_bfloat16*>(p.x) + row * p.ldx;
-    if constexpr (VEC) {
-      const uint4 g = *reinterpret_cast<const uint4*>(row_ptr + c * 8);
-      const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 a = bf2_to_f2(gw[k]);
-        y[2 * k] = a.x;
-        y[2 * k + 1] = a.y;
+        for (int k = 0; k < 8; ++k) f[k] = __bfloat162float(base[min(loose_col(c, k), p.cols - 1)]);
       }
     } else {
+      const float* base = static_cast<const float*>(p.x) + row * p.ldx;
+      if constexpr (VEC) {
+        a = reinterpret_cast<const uint4*>(base + c * 8)[0];
+        b = reinterpret_cast<const uint4*>(base + c * 8)[1];
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = loose_col(c, k) < p.cols ? __bfloat162float(row_ptr[loose_col(c, k)]) : 0.f;
-    }
-  } else {
-    const float* row_ptr = static_cast<const float*>(p.x) + row * p.ldx;
-    if constexpr (VEC) {
-      const float4 a = reinterpret_cast<const float4*>(row_ptr + c * 8)[0], b = reinterpret_cast<const float4*>(row_ptr + c * 8)[1];
-      y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
-      y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = loose_col(c, k) < p.cols ? row_ptr[loose_col(c, k)] : 0.f;
+        for (int k = 0; k < 8; ++k) f[k] = base[min(loose_col(c, k), p.cols - 1)];
+      }
     }
   }
-}
+  __device__ __forceinline__ void widen(float (&y)[8]) const {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = f[k];     // repeats of the last column do not change a maximum
+    } else if constexpr (SRC == SRC_F32) {
+      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = __uint_as_float(w[k]);
+    } else {
+      const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = bf2_to_f2(aw[k]);
+        y[2 * k] = v.x;
+        y[2 * k + 1] = v.y;
+      }
+      if constexpr (SRC == SRC_SWIGLU) {
+        const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 u = bf2_to_f2(bw[k]);
+          y[2 * k] = silu_f(y[2 * k]) * u.x;
+          y[2 * k + 1] = silu_f(y[2 * k + 1]) * u.y;
+        }
+      }
+    }
+  }
+};
 
 template <bool VEC>
 __device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, const float (&y)[8], float inv) {
@@ -217,25 +287,37 @@ __device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, c
   }
 }
 
-// blockDim = (columns / 8 covered at once, rows): every run of 16 threads in x is one group.
-template <int SRC, bool VEC>
+// blockDim = (columns / 8 covered at once, rows): every run of 16 threads in x is one group.  A thread takes
+// the same columns of UNROLL rows, all of them requested before the first is used: with one 16-byte load
+// per thread 8192 x 4096 bf16 took 21.7 us, with four 18.7 (5.4 TB/s); fp32 26 us (6.4 TB/s); SwiGLU
+// 8192 x 14336 102 and 97 us (6.0 TB/s).  Rows that allow no 16-byte vectors (8192 x 4001): 27 us.
+template <int SRC, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const RowParams p) {
   HB_LAUNCH_DEPENDENTS();
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * blockDim.y * UNROLL + threadIdx.y;
   const int c = blockIdx.y * blockDim.x + threadIdx.x;
-  const bool live = row < p.rows && (VEC ? c * 8 : loose_col(c, 0)) < p.cols;
-  float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live) load8<SRC, VEC>(p, row, c, y);
-  const float s = scale_of(group_max(abs_max8(y)));
-  if (live) {
-    store8<VEC>(p, row, c, y, 1.0f / s);
-    if ((threadIdx.x & 15) == 0) p.scale[row * p.ss0 + (c >> 4) * p.ss1] = s;
+  const bool mine = (VEC ? c * 8 : loose_col(c, 0)) < p.cols;
+  const int c_load = mine ? c : 0;
+  Values<SRC, VEC> v[UNROLL];
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) v[i].load(p, min(row0 + i * blockDim.y, p.rows - 1), c_load);
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    const int64_t row = row0 + i * blockDim.y;
+    float y[8];
+    v[i].widen(y);
+    const float s = scale_of(group_max(mine ? abs_max8(y) : 0.f));
+    if (mine && row < p.rows) {
+      store8<VEC>(p, row, c, y, inverse_of(s));
+      if ((threadIdx.x & 15) == 0) p.scale[row * p.ss0 + (c >> 4) * p.ss1] = s;
+    }
   }
 }
 
 // ------------------------------------------------------------------ 128 x 128 blocks
 // One CTA per block, 64 values per thread in registers: 16 threads span the 128 columns, 16 rows
-// are read at a time.
+// are read at a time.  Bound by HBM: 28672 x 4096 from fp32 95 us (6.2 TB/s), from bf16 56 us (6.3 TB/s; 73 us
+// while the values were widened before the maximum and so took twice the registers).
 template <int SRC, bool VEC>
 __global__ void __launch_bounds__(256) quant_blocks_kernel(const RowParams p) {
   __shared__ float red[8];
@@ -243,14 +325,16 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const RowParams p) {
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * QG + (threadIdx.x >> 4);
   const int c = blockIdx.y * (QG / 8) + (threadIdx.x & 15);
   const bool live = (VEC ? c * 8 : loose_col(c, 0)) < p.cols;
-  float y[8][8];
+  const int c_load = live ? c : 0;
+  Values<SRC, VEC> v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i].load(p, min(row0 + 16 * i, p.rows - 1), c_load);
   float m = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) y[i][k] = 0.f;
-    if (row0 + 16 * i < p.rows && live) load8<SRC, VEC>(p, row0 + 16 * i, c, y[i]);
-    m = fmaxf(m, abs_max8(y[i]));
+    float y[8];
+    v[i].widen(y);
+    if (live && row0 + 16 * i < p.rows) m = fmaxf(m, abs_max8(y));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -258,10 +342,14 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const RowParams p) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
-  const float s = scale_of(m), inv = 1.0f / s;
+  const float s = scale_of(m), inv = inverse_of(s);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (row0 + 16 * i < p.rows && live) store8<VEC>(p, row0 + 16 * i, c, y[i], inv);
+    if (row0 + 16 * i < p.rows && live) {
+      float y[8];
+      v[i].widen(y);
+      store8<VEC>(p, row0 + 16 * i, c, y, inv);
+    }
   if (threadIdx.x == 0) p.scale[blockIdx.x * p.ss0 + blockIdx.y * p.ss1] = s;
 }
 
@@ -301,9 +389,14 @@ template <int SRC, bool VEC>
 hb_status launch_rows(hb_ctx* ctx, const RowParams& p, const char* what) {
   const int64_t vecs = VEC ? p.cols / 8 : (int64_t)(p.cols + QG - 1) / QG * 16;
   const int tx = pow2_up(vecs, 16, 256), ty = 256 / tx;
-  const dim3 grid((unsigned)((p.rows + ty - 1) / ty), (unsigned)((vecs + tx - 1) / tx));
-  if (grid.y > 65535) return hb_fail(ctx, HB_ERR_UNSUPPORTED, "%s: too many columns", what);
-  const cudaError_t e = hb_launch_dependent(quant_rows_kernel<SRC, VEC>, grid, dim3(tx, ty), 0, ctx->stream, p);
+  const int64_t across = (vecs + tx - 1) / tx;
+  if (across > 65535) return hb_fail(ctx, HB_ERR_UNSUPPORTED, "%s: too many columns", what);
+  // several rows per thread once there is work for every SM with that
+  const bool many = (p.rows + 4 * ty - 1) / (4 * ty) * across >= 4 * ctx->sm_count;
+  const int rows = many ? 4 * ty : ty;
+  const dim3 grid((unsigned)((p.rows + rows - 1) / rows), (unsigned)across);
+  const cudaError_t e = hb_launch_dependent(many ? quant_rows_kernel<SRC, VEC, 4> : quant_rows_kernel<SRC, VEC, 1>, grid, dim3(tx, ty),
+                                            0, ctx->stream, p);
   if (e != cudaSuccess) { cudaGetLastError(); return hb_check_cuda(ctx, e, what); }
   ctx->launches++;
   return HB_OK;
@@ -366,23 +459,41 @@ hb_status rmsnorm_quant(hb_ctx* ctx, const hb_tensor* x, const void* gain, hb_te
   hb_status st = check_rows(ctx, op, "x", x, x->shape[0], x->shape[1]);
   if (st != HB_OK) return st;
   const int64_t rows = x->shape[0], cols = x->shape[1];
-  if (cols % 8 || cols > RMS_THREADS * RMS_MAX_VEC * 8)
-    return hb_fail(ctx, HB_ERR_UNSUPPORTED, "%s: cols must be a multiple of 8 and at most %d", op, RMS_THREADS * RMS_MAX_VEC * 8);
+  if (cols % 8 || cols > RMS_MAX_COLS)
+    return hb_fail(ctx, HB_ERR_UNSUPPORTED, "%s: cols must be a multiple of 8 and at most %d", op, RMS_MAX_COLS);
   if (res && (st = check_rows(ctx, op, "the residual", res, rows, cols)) != HB_OK) return st;
   if ((st = check_pair(ctx, op, q, scale, rows, cols, 1)) != HB_OK) return st;
   if (!aligned(x->ptr, x->stride[0] * 2, 16) || !aligned(gain, 0, 16) || (res && !aligned(res->ptr, res->stride[0] * 2, 16)) ||
       !aligned(q->ptr, q->stride[0], 8))
     return hb_fail(ctx, HB_ERR_INVALID,
                    "%s: gain and rows of x and the residual must be 16-byte aligned, rows of the output 8-byte aligned", op);
+  const int cols8 = (int)(cols / 8);
+  const int vec = cols8 <= 16 ? 1 : 2;                              // 16-byte vectors per thread
+  const int tpr = pow2_up((cols8 + vec - 1) / vec, 16, 1024);
+  const int threads = tpr > 256 ? tpr : 256;
   NormParams p = {static_cast<const __nv_bfloat16*>(x->ptr), static_cast<const uint4*>(gain),
                   res ? static_cast<__nv_bfloat16*>(res->ptr) : nullptr, static_cast<uint8_t*>(q->ptr),
-                  static_cast<float*>(scale->ptr), x->stride[0], res ? res->stride[0] : 0, q->stride[0], scale->stride[0],
-                  scale->stride[1], (int)(cols / 8), 1.0f / (float)cols, eps};
+                  static_cast<float*>(scale->ptr), rows, x->stride[0], res ? res->stride[0] : 0, q->stride[0], scale->stride[0],
+                  scale->stride[1], cols8, tpr, 1.0f / (float)cols, eps};
   hb_device_guard guard(ctx);
-  const int vec = (int)((cols / 8 + RMS_THREADS - 1) / RMS_THREADS);
-  void (*kern)(NormParams) = vec <= 1 ? rmsnorm_quant_kernel<1> : vec <= 2 ? rmsnorm_quant_kernel<2>
-                             : vec <= 4 ? rmsnorm_quant_kernel<4> : rmsnorm_quant_kernel<RMS_MAX_VEC>;
-  const cudaError_t e = hb_launch_dependent(kern, dim3((unsigned)rows), dim3(RMS_THREADS), 0, ctx->stream, p);
+  void (*kern)(NormParams);
+#define HB_NORM_PICK(T)                                                                                               \
+  kern = vec == 1 ? (res ? rmsnorm_quant_kernel<1, true, T> : rmsnorm_quant_kernel<1, false, T>)                      \
+                  : (res ? rmsnorm_quant_kernel<2, true, T> : rmsnorm_quant_kernel<2, false, T>)
+  if (threads == 256) HB_NORM_PICK(256);
+  else if (threads == 512) HB_NORM_PICK(512);
+  else HB_NORM_PICK(1024);
+#undef HB_NORM_PICK
+  static int resident[64][3][4] = {};                               // CTAs per SM, by device and variant
+  int& per_sm = resident[ctx->device & 63][threads / 512][2 * vec - 2 + (res ? 1 : 0)];
+  if (!per_sm) {
+    int n = 0;
+    HB_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0));
+    per_sm = n > 0 ? n : 1;
+  }
+  const int64_t steps = (rows + threads / tpr - 1) / (threads / tpr);
+  const int64_t most = (int64_t)ctx->sm_count * per_sm;
+  const cudaError_t e = hb_launch_dependent(kern, dim3((unsigned)(steps < most ? steps : most)), dim3(threads), 0, ctx->stream, p);
   if (e != cudaSuccess) { cudaGetLastError(); return hb_check_cuda(ctx, e, op); }
   ctx->launches++;
   return HB_OK;
