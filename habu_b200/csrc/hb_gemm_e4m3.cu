@@ -150,33 +150,123 @@ __device__ __forceinline__ void tile_coords(int tile, const TileParams& p, int& 
   tn = in_group / rows;
 }
 
-// 32 output columns of one row from col0 on, rounded once: into staging buffer `buf` of the warp (the
-// caller hands it to TMA, which writes whole lines and clips the block at the matrix edge), or
-// straight to memory where C's base, pitch or width allow no tensor map.
-__device__ __forceinline__ void put_chunk(const TileParams& p, uint32_t stage, int buf, int lane, int row0, int col0, int ncols,
-                                          const float (&f)[32]) {
-  uint32_t o[16];
+// ---- blocks of 32 rows x COLS bf16 columns in a warp's staging buffer.  COLS = 32: 64-byte rows, the
+// 16-byte piece c of row r at piece c ^ ((r >> 1) & 3), which is TMA's 64-byte swizzle; COLS = 16: plain
+// 32-byte rows.
+template <int COLS>
+__device__ __forceinline__ uint32_t piece_at(uint32_t buf, int r, int c) {
+  return buf + r * (2 * COLS) + ((COLS == 32 ? c ^ ((r >> 1) & 3) : c) << 4);
+}
+// This lane's row (row number `lane`) of a block: COLS fp32 values, rounded once.
+template <int COLS>
+__device__ __forceinline__ void put_row(uint32_t buf, int lane, const float* f) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) o[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
-  if (p.tma_store) {
-    const uint32_t mine = stage + buf * STAGE_BUF_BYTES + lane * 64;
-    const int sw = (lane >> 1) & 3;
+  for (int c = 0; c < COLS / 8; ++c)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at<COLS>(buf, lane, c)), "r"(pack_bf16x2(f[8 * c], f[8 * c + 1])),
+                 "r"(pack_bf16x2(f[8 * c + 2], f[8 * c + 3])), "r"(pack_bf16x2(f[8 * c + 4], f[8 * c + 5])),
+                 "r"(pack_bf16x2(f[8 * c + 6], f[8 * c + 7]))
+                 : "memory");
+}
+// ... and the same read back and added (the residual).
+template <int COLS>
+__device__ __forceinline__ void add_row(uint32_t buf, int lane, float* f) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mine + ((c ^ sw) << 4)), "r"(o[4 * c]), "r"(o[4 * c + 1]),
-                   "r"(o[4 * c + 2]), "r"(o[4 * c + 3])
-                   : "memory");
-  } else if (row0 + lane < p.M) {
-    __nv_bfloat16* dst = p.C + static_cast<int64_t>(row0 + lane) * p.ldc + col0;
+  for (int c = 0; c < COLS / 8; ++c) {
+    uint32_t w[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece_at<COLS>(buf, lane, c)) : "memory");
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col0 + j < ncols) dst[j] = __ushort_as_bfloat16(static_cast<unsigned short>(o[j >> 1] >> 16 * (j & 1)));
+    for (int j = 0; j < 4; ++j) {
+      f[8 * c + 2 * j] += __uint_as_float(w[j] << 16);
+      f[8 * c + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
+    }
   }
 }
+// A matrix in memory, row-major bf16; `width` bytes of it (16, 4 or 2) can be moved at once, by its base
+// and pitch.
+struct Rows {
+  uintptr_t base;
+  int64_t pitch;               // bytes
+  int rows, cols, width;
+};
+__device__ __forceinline__ Rows rows_of(const void* ptr, int64_t ld, int rows, int cols) {
+  const uintptr_t base = reinterpret_cast<uintptr_t>(ptr), both = base | static_cast<uintptr_t>(ld * 2);
+  return {base, ld * 2, rows, cols, (both & 15) == 0 ? 16 : (both & 3) == 0 ? 4 : 2};
+}
+// Copies the block at (row0, col0) between memory and a staging buffer, whole warp: neighbouring lanes
+// take neighbouring pieces of a row, so that every instruction moves contiguous bytes.  What lies
+// outside the matrix is not touched.  A row per lane, as the accumulators lie, would touch 32 lines for
+// 64 bytes: 3647 x 1420 x 298 took 69 us that way.
+template <int WIDTH>
+struct Piece;
+template <>
+struct Piece<16> { using T = uint4; };
+template <>
+struct Piece<4> { using T = uint32_t; };
+template <>
+struct Piece<2> { using T = uint16_t; };
+__device__ __forceinline__ void ld_shared(uint32_t at, uint4& v) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ld_shared(uint32_t at, uint32_t& v) { asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory"); }
+__device__ __forceinline__ void ld_shared(uint32_t at, uint16_t& v) { asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at) : "memory"); }
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_shared(uint32_t at, uint16_t v) { asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(v) : "memory"); }
 
-// The accumulators of one thread (row `row0 + lane`, HALF columns from col0 on) -> C.  The epilogue is a
-// template argument here and in the kernels: this code runs once per tile, and what it takes is mostly
-// the fetching of its instructions.
+template <int COLS, bool STORE, int WIDTH>
+__device__ __forceinline__ void move_pieces(const Rows& m, uint32_t buf, int lane, int row0, int col0) {
+  using T = typename Piece<WIDTH>::T;
+  constexpr int PER_ROW = 2 * COLS / WIDTH, ROWS = 32 / PER_ROW;    // lanes per row, rows per step
+  constexpr int STEPS = 32 / ROWS, BATCH = STEPS < 8 ? STEPS : 8;   // steps whose loads go out together
+  const int in_row = lane % PER_ROW * WIDTH, col = col0 + in_row / 2;
+  const bool whole = col + WIDTH / 2 <= m.cols;
+#pragma unroll 1
+  for (int s0 = 0; s0 < STEPS; s0 += BATCH) {
+    T v[BATCH] = {};
+    const int r0 = s0 * ROWS + lane / PER_ROW;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int r = r0 + i * ROWS;
+      if constexpr (STORE) ld_shared(piece_at<COLS>(buf, r, in_row >> 4) + (in_row & 15), v[i]);
+      else if (whole && row0 + r < m.rows) v[i] = *reinterpret_cast<const T*>(m.base + (row0 + r) * m.pitch + 2 * static_cast<int64_t>(col));
+    }
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int r = r0 + i * ROWS;
+      if constexpr (!STORE) st_shared(piece_at<COLS>(buf, r, in_row >> 4) + (in_row & 15), v[i]);
+      else if (whole && row0 + r < m.rows) *reinterpret_cast<T*>(m.base + (row0 + r) * m.pitch + 2 * static_cast<int64_t>(col)) = v[i];
+    }
+  }
+  if (WIDTH > 2 && !whole && col < m.cols) {         // the rows end inside this lane's piece
+    for (int r = lane / PER_ROW; r < 32 && row0 + r < m.rows; r += ROWS)
+      for (int j = 0; j < WIDTH / 2 && col + j < m.cols; ++j) {
+        const uint32_t at = piece_at<COLS>(buf, r, in_row >> 4) + (in_row & 15) + 2 * j;
+        uint16_t* mem = reinterpret_cast<uint16_t*>(m.base + (row0 + r) * m.pitch + 2 * static_cast<int64_t>(col + j));
+        uint16_t v;
+        if constexpr (STORE) {
+          ld_shared(at, v);
+          *mem = v;
+        } else {
+          v = *mem;
+          st_shared(at, v);
+        }
+      }
+  }
+}
+template <int COLS, bool STORE>
+__device__ __forceinline__ void move_block(const Rows& m, uint32_t buf, int lane, int row0, int col0) {
+  if (m.width == 16) move_pieces<COLS, STORE, 16>(m, buf, lane, row0, col0);
+  else if (m.width == 4) move_pieces<COLS, STORE, 4>(m, buf, lane, row0, col0);
+  else move_pieces<COLS, STORE, 2>(m, buf, lane, row0, col0);
+}
+
+// The accumulators of one thread (row `row0 + lane`, HALF columns from col0 on) -> C: rounded once into
+// the warp's staging buffers, and from there by TMA (whole lines, clipped at the matrix edge) or, where
+// C's base, pitch or width allow no tensor map, by the warp.  The epilogue is a template argument here
+// and in the kernels: this code runs once per tile, and what it takes is mostly the fetching of its
+// instructions.
 template <int EPI, int HALF>
 __device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMap* tmC, uint32_t stage, int lane, int row0,
                                            int col0, const uint64_t (&acc)[HALF / 2]) {
@@ -185,65 +275,51 @@ __device__ __forceinline__ void write_half(const TileParams& p, const CUtensorMa
     __syncwarp();
   }
   constexpr bool swiglu = EPI == HB_EPI_SWIGLU;
-  if constexpr (swiglu) {
-    // columns interleave (gate, up): 64 sums give 32 outputs
+  constexpr int BLOCKS = swiglu ? HALF / 64 : HALF / 32;
+  const int first = swiglu ? col0 >> 1 : col0, ncols = swiglu ? p.N >> 1 : p.N;
+  if constexpr (EPI == HB_EPI_RESIDUAL) {
+    const Rows r = rows_of(p.R, p.ldr, p.M, p.N);
+    for (int c = 0; c < BLOCKS; ++c) move_block<32, false>(r, stage + c * STAGE_BUF_BYTES, lane, row0, first + c * 32);
+    __syncwarp();
+  }
 #pragma unroll
-    for (int c = 0; c < HALF / 64; ++c) {
-      float f[32];
+  for (int c = 0; c < BLOCKS; ++c) {
+    const uint32_t buf = stage + c * STAGE_BUF_BYTES;
+    float f[32];
+    if constexpr (swiglu) {                        // columns interleave (gate, up): 64 sums give 32 outputs
 #pragma unroll
       for (int j = 0; j < 32; ++j) {
         const float2 gu = unpack2(acc[c * 32 + j]);
         f[j] = silu(gu.x) * gu.y;
       }
-      put_chunk(p, stage, c, lane, row0, (col0 >> 1) + c * 32, p.N >> 1, f);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < HALF / 32; ++c) {
-      float f[32];
+    } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const float2 v = unpack2(acc[c * 16 + j]);
         f[2 * j] = v.x;
         f[2 * j + 1] = v.y;
       }
-      const int col = col0 + c * 32;
-      if constexpr (EPI == HB_EPI_GELU) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
-      }
-      if (EPI == HB_EPI_RESIDUAL && row0 + lane < p.M) {
-        const __nv_bfloat16* r = p.R + static_cast<int64_t>(row0 + lane) * p.ldr + col;
-        if ((p.ldr & 7) == 0 && (reinterpret_cast<uintptr_t>(p.R) & 15) == 0 && col + 32 <= p.N) {
-#pragma unroll
-          for (int j4 = 0; j4 < 4; ++j4) {
-            const uint4 rv = *(reinterpret_cast<const uint4*>(r) + j4);
-            const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              f[j4 * 8 + 2 * j] += __uint_as_float(rw[j] << 16);
-              f[j4 * 8 + 2 * j + 1] += __uint_as_float(rw[j] & 0xffff0000u);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j < p.N) f[j] += __bfloat162float(r[j]);
-        }
-      }
-      put_chunk(p, stage, c, lane, row0, col, p.N, f);
     }
+    if constexpr (EPI == HB_EPI_GELU) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) f[j] = gelu_erf(f[j]);
+    }
+    if constexpr (EPI == HB_EPI_RESIDUAL) add_row<32>(buf, lane, f);
+    put_row<32>(buf, lane, f);
   }
   if (p.tma_store) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0 && row0 < p.M) {
-      const int first = swiglu ? col0 >> 1 : col0, ncols = swiglu ? p.N >> 1 : p.N;
-      const int n = swiglu ? HALF / 64 : HALF / 32;
-      for (int c = 0; c < n; ++c)
+      for (int c = 0; c < BLOCKS; ++c)
         if (first + c * 32 < ncols) tma_store_2d(tmC, stage + c * STAGE_BUF_BYTES, first + c * 32, row0);
       tma_store_commit();
     }
+  } else {
+    __syncwarp();
+    const Rows out = rows_of(p.C, p.ldc, p.M, ncols);
+    for (int c = 0; c < BLOCKS; ++c) move_block<32, true>(out, stage + c * STAGE_BUF_BYTES, lane, row0, first + c * 32);
+    __syncwarp();                                  // the buffers are rewritten by the next tile
   }
 }
 
@@ -276,15 +352,13 @@ __device__ __forceinline__ void st_cluster_v4(uint32_t addr, float4 v) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
 }
 
-// Sixteen finished sums of row `row` from column col0 on: epilogue, one rounding, stores of the row's own
-// bytes (a tile that is split is one of few, and its output small).
+// Sixteen finished sums of row `row0 + lane` from column col0 on -> C, by way of the warp's staging buffer
+// (a tile that is split is one of few, and its output small: no TMA).
 template <int EPI>
-__device__ __forceinline__ void put16(const TileParams& p, int row, int col0, float (&f)[16]) {
-  if (row >= p.M) return;
+__device__ __forceinline__ void put16(const TileParams& p, uint32_t stage, int lane, int row0, int col0, float (&f)[16]) {
   constexpr bool swiglu = EPI == HB_EPI_SWIGLU;
-  constexpr int OUT = swiglu ? 8 : 16;
-  const int first = swiglu ? col0 >> 1 : col0, ncols = swiglu ? p.N >> 1 : p.N;
-  if constexpr (swiglu) {                          // columns interleave (gate, up)
+  __syncwarp();                                    // the buffer may still be read for the last piece
+  if constexpr (swiglu) {                          // columns interleave (gate, up): eight outputs
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = silu(f[2 * j]) * f[2 * j + 1];
   }
@@ -292,36 +366,15 @@ __device__ __forceinline__ void put16(const TileParams& p, int row, int col0, fl
 #pragma unroll
     for (int j = 0; j < 16; ++j) f[j] = gelu_erf(f[j]);
   }
+  const int first = swiglu ? col0 >> 1 : col0, ncols = swiglu ? p.N >> 1 : p.N;
   if constexpr (EPI == HB_EPI_RESIDUAL) {
-    const __nv_bfloat16* r = p.R + static_cast<int64_t>(row) * p.ldr + first;
-    if (first + 16 <= ncols && (reinterpret_cast<uintptr_t>(r) & 15) == 0) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4 rv = reinterpret_cast<const uint4*>(r)[h];
-        const uint32_t rw[4] = {rv.x, rv.y, rv.z, rv.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[8 * h + 2 * j] += __uint_as_float(rw[j] << 16);
-          f[8 * h + 2 * j + 1] += __uint_as_float(rw[j] & 0xffff0000u);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (first + j < ncols) f[j] += __bfloat162float(r[j]);
-    }
+    move_block<16, false>(rows_of(p.R, p.ldr, p.M, p.N), stage, lane, row0, first);
+    __syncwarp();
+    add_row<16>(stage, lane, f);
   }
-  __nv_bfloat16* dst = p.C + static_cast<int64_t>(row) * p.ldc + first;
-  if (first + OUT <= ncols && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-#pragma unroll
-    for (int h = 0; h < OUT / 8; ++h)
-      reinterpret_cast<uint4*>(dst)[h] = make_uint4(pack_bf16x2(f[8 * h], f[8 * h + 1]), pack_bf16x2(f[8 * h + 2], f[8 * h + 3]),
-                                                    pack_bf16x2(f[8 * h + 4], f[8 * h + 5]), pack_bf16x2(f[8 * h + 6], f[8 * h + 7]));
-  } else {
-#pragma unroll
-    for (int j = 0; j < OUT; ++j)
-      if (first + j < ncols) dst[j] = __float2bfloat16_rn(f[j]);
-  }
+  put_row<16>(stage, lane, f);
+  __syncwarp();
+  move_block<16, true>(rows_of(p.C, p.ldc, p.M, swiglu ? min(ncols, first + 8) : ncols), stage, lane, row0, first);
 }
 
 template <int KIND, int BN, int STAGES, int EPI>
@@ -552,7 +605,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
               f[4 * j] += v.x; f[4 * j + 1] += v.y; f[4 * j + 2] += v.z; f[4 * j + 3] += v.w;
             }
           }
-          put16<EPI>(p, row0 + lane, col0 + c * 16, f);
+          put16<EPI>(p, stage_mine, lane, row0, col0 + c * 16, f);
         }
       } else {
         if (ok) write_half<EPI, HALF>(p, &tmC, stage_mine, lane, row0, col0, acc);

@@ -403,3 +403,142 @@ def test_a_feed_forward_sublayer(ctx, rows):
     assert np.all(np.abs(got - want) <= qr.product_tolerance(av, w2v, want))
     for t in (dw1, dw2, q1, s1, q2, s2, dx, dr, dg, h, hs, gu, a, as_, out):
         ctx.free(t)
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """Rows more than 2^31 elements apart: every row index is multiplied by its pitch in 64 bits.  The
+    operators touch a few rows of a buffer that is otherwise left alone."""
+    far = (1 << 31) + 64
+    rows, cols, N = 3, 256, 300
+    rng = np.random.default_rng(9)
+    x, xb = _bf16(rng, (rows, cols))
+    r, rb = _bf16(rng, (rows, cols))
+    g, gb = _bf16(rng, (cols,))
+    bx, bq, bc = ctx.empty((2 * far + 1024,)), ctx.empty((2 * far + 1024,), hb.HB_E4M3), ctx.empty((2 * far + 1024,))
+    dx = ctx.wrap(bx.ptr, (rows, cols), hb.HB_BF16, (far, 1))
+    dr = ctx.wrap(bc.ptr, (rows, cols), hb.HB_BF16, (far, 1))
+    dq = ctx.wrap(bq.ptr, (rows, cols), hb.HB_E4M3, (far, 1))
+    for i in range(rows):
+        _up(ctx, bx.ptr + 2 * i * far, xb[i])
+        _up(ctx, bc.ptr + 2 * i * far, rb[i])
+
+    def fetch(buf, elem, dtype, width):
+        return np.stack([ctx.download(ctx.wrap(buf.ptr + elem * i * far, (width,), dtype)) for i in range(rows)])
+    _, s = ctx.quantize(dx, dq, None, 1)
+    qr.check_pair(x.astype(np.float64), fetch(bq, 1, hb.HB_E4M3, cols), ctx.download(s), 1, 0.0)
+    _, s = ctx.quantize(dx, dq, None, 128)
+    qr.check_pair(x.astype(np.float64), fetch(bq, 1, hb.HB_E4M3, cols), ctx.download(s), 128, 0.0)
+    _, s = ctx.swiglu_quant(dx, ctx.wrap(bq.ptr, (rows, cols // 2), hb.HB_E4M3, (far, 1)))
+    qr.check_pair(qr.swiglu(x), fetch(bq, 1, hb.HB_E4M3, cols // 2), ctx.download(s), 1, 2.0 ** -18)
+    _, s = ctx.rmsnorm_quant(dx, ctx.upload(gb), dq, residual=dr)
+    base = oracle.round_bf16((x.astype(np.float64) + r).astype(np.float32))
+    assert np.array_equal(fetch(bc, 2, hb.HB_BF16, cols), oracle.to_bf16_bits(base))
+    ab = fetch(bq, 1, hb.HB_E4M3, cols)
+    sa = ctx.download(s)
+    qr.check_pair(qr.rmsnorm(base, g.astype(np.float64), 1e-5), ab, sa, 1, 2.0 ** -17)
+    # the product: A, the residual and C with that pitch, and B for the few-row kernel
+    av = qr.decode(ab) * qr.spread(sa.astype(np.float64), rows, cols, 1)
+    bb, sb, bv = qr.operands(rng, N, cols, 128)
+    B, SB = _upload_pair(ctx, bb, sb)
+    dc = ctx.wrap(bx.ptr, (rows, N), hb.HB_BF16, (far, 1))
+    for i in range(rows):
+        _up(ctx, bc.ptr + 2 * i * far, oracle.to_bf16_bits(np.zeros(N, np.float32) + i))
+    ctx.matmul_scaled(dq, s, B.T, SB.T, dc, epilogue=hb.HB_EPI_RESIDUAL, residual=ctx.wrap(bc.ptr, (rows, N), hb.HB_BF16, (far, 1)))
+    want = av @ bv.T + np.arange(rows)[:, None]
+    got = oracle.from_bf16_bits(fetch(bx, 2, hb.HB_BF16, N)).astype(np.float64)
+    assert np.all(np.abs(got - want) <= qr.product_tolerance(av, bv, want) + np.abs(want) * 2.0 ** -23)
+    # roles exchanged: the far-pitched matrix as B (three columns of C), 200 rows of A: the tile kernels
+    ab2, sa2, av2 = qr.operands(rng, 200, cols, 1)
+    A2, SA2 = _upload_pair(ctx, ab2, sa2)
+    bs = ctx.upload(np.full((1, 2), 0.5, np.float32))
+    c2 = ctx.matmul_scaled(A2, SA2, dq.T, bs.T)
+    bv2 = qr.decode(ab) * 0.5
+    want = av2 @ bv2.T
+    got = oracle.from_bf16_bits(ctx.download(c2)).astype(np.float64)
+    assert np.all(np.abs(got - want) <= qr.product_tolerance(av2, bv2, want))
+    for t in (bx, bq, bc):
+        ctx.free(t)
+    _free(ctx, B, SB, A2, SA2)
+
+
+@pytest.mark.parametrize("M", [3, 90, 700])
+@pytest.mark.parametrize("N", [301, 302, 304])
+@pytest.mark.parametrize("epi", [hb.HB_EPI_NONE, hb.HB_EPI_RESIDUAL])
+def test_matmul_scaled_output_alignments(ctx, M, N, epi):
+    """Outputs and residuals whose rows start on 16, 4 or 2 bytes, in every combination that a pitch and a
+    start allow: 16-, 4- and 2-byte pieces, and TMA where it is possible."""
+    K = 2304
+    rng = np.random.default_rng(N + M)
+    ab, sa, av = qr.operands(rng, M, K, 1)
+    bb, sb, bv = qr.operands(rng, N, K, 128)
+    acc = av @ bv.T
+    A, SA = _upload_pair(ctx, ab, sa)
+    B, SB = _upload_pair(ctx, bb, sb)
+    for pad, shift in ((0, 0), (8 - N % 8, 0), (2 - N % 2, 0), (8 - N % 8, 2), (1 - N % 2, 1)):
+        c = COut(ctx, M, N, pad, shift)
+        res, want = None, acc
+        if epi == hb.HB_EPI_RESIDUAL:
+            r, rb = _bf16(rng, (M, N + pad))
+            rbuf = ctx.upload(np.concatenate([np.full(shift, 0x7FC0, np.uint16), rb.reshape(-1)]))
+            res = ctx.wrap(rbuf.ptr + 2 * shift, (M, N), hb.HB_BF16, (N + pad, 1))
+            want = acc + r[:, :N]
+        ctx.matmul_scaled(A, SA, B.T, SB.T, c.t, epilogue=epi, residual=res)
+        got = c.finish()
+        tol = qr.product_tolerance(av, bv, want) + np.abs(want) * 2.0 ** -23
+        assert np.all(np.abs(got - want) <= tol), (pad, shift)
+    _free(ctx, A, SA, B, SB)
+
+
+def test_operators_follow_the_context_stream(ctx):
+    """On a caller's stream, and back: ordered with what the caller queues there."""
+    torch = pytest.importorskip("torch")
+    rows, d, N = 64, 512, 640
+    rng = np.random.default_rng(11)
+    gb = _bf16(rng, (d,))[1]
+    dg = ctx.upload(gb)
+    w = ctx.quantize(ctx.upload(rng.standard_normal((N, d)).astype(np.float32)), block_rows=128)
+    ctx.sync()
+    st = torch.cuda.Stream()
+    ctx.set_stream(st.cuda_stream)
+    try:
+        with torch.cuda.stream(st):
+            x = torch.zeros(rows, d, device="cuda", dtype=torch.bfloat16)
+            outs = []
+            for i in range(6):
+                x += 1 + i                                # queued on the same stream, in front of the norm
+                x[:, i] = -3
+                t = ctx.wrap(x.data_ptr(), (rows, d), hb.HB_BF16)
+                h = ctx.rmsnorm_quant(t, dg)
+                outs.append((x.clone(), ctx.matmul_scaled(*h, w[0].T, w[1].T, weights=True)))
+        st.synchronize()
+    finally:
+        ctx.set_stream(None)
+    for xi, o in outs:
+        t = ctx.wrap(xi.data_ptr(), (rows, d), hb.HB_BF16)
+        h = ctx.rmsnorm_quant(t, dg)
+        again = ctx.matmul_scaled(*h, w[0].T, w[1].T)
+        assert np.array_equal(ctx.download(o), ctx.download(again))
+
+
+def test_two_contexts_at_once():
+    """Nothing is shared between contexts, and the product keeps no scratch at all: two contexts on their
+    own streams, working at the same time."""
+    rng = np.random.default_rng(12)
+    M, N, K = 16, 1024, 4096
+    cs = [hb.Context(0), hb.Context(0)]
+    work = []
+    for c in cs:
+        ab, sa, av = qr.operands(rng, M, K, 1)
+        bb, sb, bv = qr.operands(rng, N, K, 128)
+        A, SA = _upload_pair(c, ab, sa)
+        B, SB = _upload_pair(c, bb, sb)
+        work.append((c, A, SA, B, SB, av @ bv.T, qr.product_tolerance(av, bv, av @ bv.T), [c.empty((M, N)) for _ in range(20)]))
+    for i in range(20):
+        for c, A, SA, B, SB, _, _, outs in work:
+            c.matmul_scaled(A, SA, B.T, SB.T, outs[i], weights=True)
+    for c, *_, want, tol, outs in work:
+        for o in outs:
+            got = oracle.from_bf16_bits(c.download(o)).astype(np.float64)
+            assert np.all(np.abs(got - want) <= tol)
+    for c in cs:
+        c.close()
