@@ -6,8 +6,7 @@
 //   scale = max(max|y| / 448, 2^-126)     q = e4m3(y / scale)
 //
 // The floor keeps the scale normal and its reciprocal finite, so that a group of zeros (or of
-// values so small that 1 / scale would overflow) needs no case of its own.  y / scale is formed as
-// y * (1 / scale): 2^-22 off at most, against the 2^-4 of the rounding to e4m3 that follows.
+// values so small that 1 / scale would overflow) needs no case of its own.
 // fmaxf drops NaNs, so a NaN does not spread over its group: its own product is NaN and converts
 // to the e4m3 NaN.
 #include <cuda_fp8.h>
@@ -54,13 +53,24 @@ __device__ __forceinline__ float group_max(float v) {
   for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// One multiplication by fl(1 / 448) (2^-23 off at most) and an approximate reciprocal (1 ulp): a division
-// each would be a fifth of the instructions of these kernels.
-__device__ __forceinline__ float scale_of(float amax) { return fmaxf(amax * (1.0f / Q_TOP), Q_FLOOR); }
-__device__ __forceinline__ float inverse_of(float scale) {
+__device__ __forceinline__ float rcp_approx(float v) {      // 1 ulp
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(scale));
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+// What a group with maximum `top` is stored with: its scale, and the factor that takes a value to q's
+// range, q = e4m3(y * to_q).  The factor is 448 / top to within a rounding (a reciprocal and one
+// correction: a division each for the scale and its inverse would be a fifth of the instructions of
+// these kernels), at most 2^126, which is where the scale meets its floor; a group of zeros gets there by
+// way of a NaN that fminf drops.  Behind an infinity it is 0.
+struct Scale {
+  float s, to_q;
+};
+__device__ __forceinline__ Scale scale_of(float top) {
+  const float r = rcp_approx(top), k = Q_TOP * r;
+  const float exact = fmaf(fmaf(-top, k, Q_TOP), r, k);
+  return {fmaxf(top * (1.0f / Q_TOP), Q_FLOOR),                // 2^-23 off at most
+          top < INFINITY ? fminf(exact, 1.0f / Q_FLOOR) : 0.0f};
 }
 
 __device__ __forceinline__ float abs_max8(const float (&y)[8]) {
@@ -70,11 +80,11 @@ __device__ __forceinline__ float abs_max8(const float (&y)[8]) {
   return m;
 }
 // Eight values to eight e4m3 bytes (to nearest even; beyond 448 saturates, NaN stays NaN).
-__device__ __forceinline__ uint2 pack8(const float (&y)[8], float inv) {
+__device__ __forceinline__ uint2 pack8(const float (&y)[8], const Scale& z) {
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const float2 k = make_float2(inv, inv);
+    const float2 k = make_float2(z.to_q, z.to_q);
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(mul2(make_float2(y[4 * h], y[4 * h + 1]), k), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(mul2(make_float2(y[4 * h + 2], y[4 * h + 3]), k), __NV_SATFINITE, __NV_E4M3);
     w[h] = lo | hi << 16;
@@ -88,8 +98,8 @@ __device__ __forceinline__ uint2 pack8(const float (&y)[8], float inv) {
 // next rows are on their way while the statistics of these are formed, and the gain is read once.
 // With h = x * gain, y = h * r and max|y| = max|h| * r for the row's r = rsqrt(..): the maxima of the groups
 // (sixteen neighbouring threads hold one: four shuffles) do not wait for the statistic.
-// Measured: 8192 x 4096 with the residual 37.6 us (6.2 TB/s, 95 % of a copy), without it 25.6 us (bound by
-// the instructions: 3.9 TB/s), 16 x 4096 2.2 us.  One CTA per row without the prefetch: 42.1 and 30.1 us.
+// Measured: 8192 x 4096 with the residual 37.8 us (6.2 TB/s, 95 % of a copy), without it 26.6 us (bound by
+// the instructions: 3.8 TB/s), 16 x 4096 2.2 us.  One CTA per row without the prefetch: 42.1 and 30.1 us.
 constexpr int RMS_MAX_COLS = 16384;
 
 struct NormParams {
@@ -179,16 +189,15 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
       for (int i = 0; i < VEC; ++i) {
         const int c = t + i * tpr;
         if (c < p.cols8) {
-          const float s = scale_of(top[i] * inv_rms);
-          // (two products: r / scale on its own would overflow for a group of zeros)
+          const Scale z = scale_of(top[i] * inv_rms);
 #pragma unroll
           for (int k = 0; k < 8; k += 2) {
             const float2 y = mul2(make_float2(h[i][k], h[i][k + 1]), make_float2(inv_rms, inv_rms));
             h[i][k] = y.x;
             h[i][k + 1] = y.y;
           }
-          *reinterpret_cast<uint2*>(qr + c * 8) = pack8(h[i], inverse_of(s));
-          if ((c & 15) == 0) sr[(c >> 4) * p.ss1] = s;
+          *reinterpret_cast<uint2*>(qr + c * 8) = pack8(h[i], z);
+          if ((c & 15) == 0) sr[(c >> 4) * p.ss1] = z.s;
         }
       }
     }
@@ -207,8 +216,9 @@ struct RowParams {
   int cols;                    // columns of q (SwiGLU: half the columns of x)
 };
 
-// v / (1 + exp(-v)): approximate exponential and division (2 ulp each); for v far below zero the
-// denominator is infinite and the quotient -0.
+// v / (1 + exp(-v)): approximate exponential and division, 2^-21 off at most for |v| < 20 (the accurate
+// ones took SwiGLU of 8192 x 14336 from 97 to 149 us); far below zero the denominator is infinite and the
+// quotient -0.
 __device__ __forceinline__ float silu_f(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 
 // Eight values of `row` that belong to thread c of the row.  VEC: the consecutive columns 8 c .. 8 c + 7
@@ -275,9 +285,9 @@ struct Values {
 };
 
 template <bool VEC>
-__device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, const float (&y)[8], float inv) {
+__device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, const float (&y)[8], const Scale& z) {
   uint8_t* dst = p.q + row * p.ldq;
-  const uint2 w = pack8(y, inv);
+  const uint2 w = pack8(y, z);
   if constexpr (VEC) {
     *reinterpret_cast<uint2*>(dst + c * 8) = w;
   } else {
@@ -289,8 +299,8 @@ __device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, c
 
 // blockDim = (columns / 8 covered at once, rows): every run of 16 threads in x is one group.  A thread takes
 // the same columns of UNROLL rows, all of them requested before the first is used: with one 16-byte load
-// per thread 8192 x 4096 bf16 took 21.7 us, with four 18.7 (5.4 TB/s); fp32 26 us (6.4 TB/s); SwiGLU
-// 8192 x 14336 102 and 97 us (6.0 TB/s).  Rows that allow no 16-byte vectors (8192 x 4001): 27 us.
+// per thread 8192 x 4096 bf16 took 21.7 us, with four 19.2 (5.3 TB/s); fp32 27 us (6.2 TB/s); SwiGLU
+// 8192 x 14336 100 us (5.9 TB/s).  Rows that allow no 16-byte vectors (8192 x 4001): 28 us.
 template <int SRC, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const RowParams p) {
   HB_LAUNCH_DEPENDENTS();
@@ -306,10 +316,10 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const RowParams p) {
     const int64_t row = row0 + i * blockDim.y;
     float y[8];
     v[i].widen(y);
-    const float s = scale_of(group_max(mine ? abs_max8(y) : 0.f));
+    const Scale z = scale_of(group_max(mine ? abs_max8(y) : 0.f));
     if (mine && row < p.rows) {
-      store8<VEC>(p, row, c, y, inverse_of(s));
-      if ((threadIdx.x & 15) == 0) p.scale[row * p.ss0 + (c >> 4) * p.ss1] = s;
+      store8<VEC>(p, row, c, y, z);
+      if ((threadIdx.x & 15) == 0) p.scale[row * p.ss0 + (c >> 4) * p.ss1] = z.s;
     }
   }
 }
@@ -342,15 +352,15 @@ __global__ void __launch_bounds__(256) quant_blocks_kernel(const RowParams p) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
-  const float s = scale_of(m), inv = inverse_of(s);
+  const Scale z = scale_of(m);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (row0 + 16 * i < p.rows && live) {
       float y[8];
       v[i].widen(y);
-      store8<VEC>(p, row0 + 16 * i, c, y, inv);
+      store8<VEC>(p, row0 + 16 * i, c, y, z);
     }
-  if (threadIdx.x == 0) p.scale[blockIdx.x * p.ss0 + blockIdx.y * p.ss1] = s;
+  if (threadIdx.x == 0) p.scale[blockIdx.x * p.ss0 + blockIdx.y * p.ss1] = z.s;
 }
 
 bool aligned(const void* ptr, int64_t pitch_bytes, int n) {

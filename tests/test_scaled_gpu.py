@@ -542,3 +542,18 @@ def test_two_contexts_at_once():
             assert np.all(np.abs(got - want) <= tol)
     for c in cs:
         c.close()
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_around_the_floor(ctx, block_rows):
+    """Groups whose largest value runs from far below 448 x 2^-126, where the scale meets its floor, to far
+    above it: the pair stands for the values on both sides."""
+    rows, cols = 256, 128
+    rng = np.random.default_rng(13)
+    top = 2.0 ** np.linspace(-149, -100, rows if block_rows == 1 else 2)
+    y = rng.uniform(-1, 1, (rows, cols)) * np.repeat(top, rows // len(top))[:, None]
+    x = y.astype(np.float32)
+    q, s = ctx.quantize(ctx.upload(x), block_rows=block_rows)
+    bits, sc = _pitched(ctx, q), ctx.download(s)
+    assert not np.isnan(qr.decode(bits)).any()
+    qr.check_pair(x.astype(np.float64), bits, sc, block_rows, 0.0)
