@@ -225,8 +225,14 @@ hb_status hb_make_tensor_map(hb_ctx* ctx, CUtensorMap* out, CUtensorMapDataType 
   memset(&key, 0, sizeof(key));
   key.base = base; key.dt = (int32_t)dt; key.rank = rank; key.swizzle = (int32_t)swizzle;
   for (int i = 0; i < rank; ++i) { key.dims[i] = dims[i]; key.box[i] = box[i]; if (i + 1 < rank) key.strides[i] = strides_bytes[i]; }
-  uint64_t h = 1469598103934665603ull;                   // FNV-1a over the key
-  for (size_t i = 0; i < sizeof(key); ++i) { h ^= reinterpret_cast<const unsigned char*>(&key)[i]; h *= 1099511628211ull; }
+  uint64_t h = 1469598103934665603ull;                   // FNV-1a over the key, eight bytes at a time
+  static_assert(sizeof(key) % 8 == 0, "whole words");
+  for (size_t i = 0; i < sizeof(key); i += 8) {
+    uint64_t w;
+    memcpy(&w, reinterpret_cast<const unsigned char*>(&key) + i, 8);
+    h = (h ^ w) * 1099511628211ull;
+    h ^= h >> 29;                                        // the low bits of a pointer or size reach all of the hash
+  }
   if (ctx) {
     auto range = ctx->tmap_cache.equal_range(h);
     for (auto it = range.first; it != range.second; ++it)
