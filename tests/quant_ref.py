@@ -60,17 +60,18 @@ def scales(y, block_rows):
     return np.maximum(s / TOP, FLOOR)
 
 
-def check_pair(y, bits, s, block_rows, rel):
+def check_pair(y, bits, s, block_rows, rel, t_abs=0.0):
     """`bits`, `s` are what the device made of y.  `rel` bounds the relative error of the fp32
     arithmetic in front of the rounding: of y itself, and of the maximum.  The scale adds one
     division (2^-24) and y / scale a reciprocal and a product (2^-24 each), so the value that is
-    rounded is off by at most 2 rel + 2^-22 of itself, and q by half an e4m3 step beside that."""
+    rounded is off by at most 2 rel + 2^-22 of itself, and q by half an e4m3 step beside that.  `t_abs`
+    bounds what subnormal values in front of the rounding lose, in units of q."""
     rows, cols = y.shape
     want = scales(y, block_rows)
-    assert np.all(np.abs(s - want) <= want * (rel + 2.0 ** -23)), "scale"
+    assert np.all(np.abs(s - want) <= want * (rel + 2.0 ** -23 + t_abs / TOP)), "scale"
     t = y / spread(np.asarray(s, np.float64), rows, cols, block_rows)
     q = decode(bits)
-    off = np.abs(q - np.clip(t, -TOP, TOP)) - half_step(t) - np.abs(t) * (2 * rel + 2.0 ** -22)
+    off = np.abs(q - np.clip(t, -TOP, TOP)) - half_step(t) - np.abs(t) * (2 * rel + 2.0 ** -22) - t_abs
     assert np.all(off <= 0), f"q is {off.max()} beyond the nearest value"
 
 

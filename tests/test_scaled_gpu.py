@@ -557,3 +557,37 @@ def test_quantize_around_the_floor(ctx, block_rows):
     bits, sc = _pitched(ctx, q), ctx.download(s)
     assert not np.isnan(qr.decode(bits)).any()
     qr.check_pair(x.astype(np.float64), bits, sc, block_rows, 0.0)
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,cols", [(37, 256), (5, 2560), (300, 1920), (3, 10240)])
+def test_rmsnorm_quant_around_the_floor(ctx, rows, cols, residual):
+    """Gains that take whole groups from far below the floor of the scale to far above it, beside rows of
+    zeros, of a statistic that overflows, and with a NaN or an infinity."""
+    rng = np.random.default_rng(rows)
+    x, xb = _bf16(rng, (rows, cols))
+    g, gb = _bf16(rng, (cols,))
+    g *= np.repeat(2.0 ** np.linspace(-133, -100, cols // 128).round(), 128)
+    gb = oracle.to_bf16_bits(g.astype(np.float32))
+    g = oracle.round_bf16(g.astype(np.float32)).astype(np.float64)
+    x[0], xb[0] = 0, 0
+    huge = 2.0 ** 100                # squares beyond fp32: the root's inverse is 0
+    xb[1] = oracle.to_bf16_bits((x[1] * huge).astype(np.float32))
+    xb[2, cols - 1] = 0x7FC0
+    if rows > 3:
+        xb[3, 5] = 0xFF80            # minus infinity
+    dx, dr = ctx.upload(xb), ctx.upload(np.zeros((rows, cols), np.uint16))
+    out = Out(ctx, rows, cols, 1, 16, False)
+    ctx.rmsnorm_quant(dx, ctx.upload(gb), out.q, out.scale, 1e-5, dr if residual else None)
+    q, s = out.finish()
+    if residual:
+        assert np.array_equal(ctx.download(dr)[[0, 1]], xb[[0, 1]])
+    v = qr.decode(q)
+    assert (v[0] == 0).all() and (v[1] == 0).all() and (s[:2] == np.float32(qr.FLOOR)).all()
+    assert np.isnan(v[2]).all()
+    if rows > 3:
+        assert np.isnan(v[3, 5]) and (np.delete(v[3], 5) == 0).all()
+    # x * gain is formed first: below 2^-126 it is off by 2^-150, which the root's inverse (at most 1.2 for
+    # rows of unit variance) and a scale of 2^-126 or more turn into 1.2 * 2^-24 units of q
+    good = [0] + list(range(4, rows))
+    qr.check_pair(qr.rmsnorm(x[good], g, 1e-5), q[good], s[good], 1, 2.0 ** -17, 2.0 ** -23)
