@@ -108,12 +108,10 @@ __device__ __forceinline__ uint2 pack8(const float (&y)[8], const Scale& z) {
 // With h = x * gain, y = h * r and max|y| = max|h| * r for the row's r = rsqrt(..): y / scale = h * 448 / max|h|
 // does not depend on the row's statistic.  So a vector is done with at once and no row stays in registers;
 // the scales come behind, for BATCH rows at a time: one barrier, and one thread per group adds up the
-// row's sum (a barrier per row, with one warp at the scales and the others waiting for it: 23.0 for 20.9 us
-// below).  Where y / scale is not that (the scale meets its floor, r or a maximum is not finite), that
+// row's sum (a barrier per row, with one warp at the scales and the others waiting for it: a tenth slower).  Where y / scale is not that (the scale meets its floor, r or a maximum is not finite), that
 // thread forms the group's q again, from y.
-// Bound by HBM with the residual: 8192 x 4096 37.8 us (6.2 TB/s, 95 % of a copy).  Without it 20.9 us (4.8 TB/s):
-// some 110 instructions per 256 values, a third of them the widening of x and the packing of q; 16 x 4096
-// 2.2 us.  With y in registers until the statistic was there, q formed from it: 37.9 and 26.5 us.
+// Bound by HBM with the residual: 8192 x 4096 37.8 us (6.2 TB/s, 95 % of a copy).  Without it 20.0 us (5.0 TB/s),
+// bound by its instructions (118 per warp and 256 values; 69 % of the issue slots taken); 16 x 4096 2.1 us.  With y in registers until the statistic was there, q formed from it: 37.9 and 26.5 us.
 constexpr int RMS_MAX_COLS = 16384;
 
 struct NormParams {
@@ -122,9 +120,9 @@ struct NormParams {
   __nv_bfloat16* residual;     // or null
   uint8_t* q;
   float* scale;
-  int64_t rows;
-  int64_t ldx, ldr, ldq, ss0, ss1;
-  int cols8, tpr;
+  uint32_t rows;               // row numbers in 32 bits, offsets in 64: one wide multiply-add each
+  uint64_t ldx, ldr, ldq, ss0, ss1;
+  uint32_t cols8, tpr;
   float inv_cols, eps;
 };
 
@@ -142,17 +140,17 @@ template <int VEC, bool RES, int THREADS>
 __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams p) {
   using L = NormLayout<VEC, RES, THREADS>;
   extern __shared__ uint4 places[];
-  constexpr int BATCH = L::BATCH, SLOTS = THREADS / 16 * VEC;
+  constexpr uint32_t BATCH = L::BATCH, SLOTS = THREADS / 16 * VEC;
   static_assert(BATCH * SLOTS <= THREADS, "one thread per group of a batch");
   __shared__ float red[2][BATCH][THREADS / 16], tops[2][BATCH][SLOTS];
-  const int tpr = p.tpr, warps = tpr > 32 ? tpr / 32 : 1;           // warps that share a row
-  const int t = threadIdx.x & (tpr - 1);                            // thread of the row
-  const int sub_row = threadIdx.x / tpr, per_step = THREADS / tpr;
-  const int groups = (p.cols8 + 15) >> 4, row_slots = (tpr >> 4) * VEC;
+  const uint32_t tpr = p.tpr, warps = tpr > 32 ? tpr / 32 : 1;           // warps that share a row
+  const uint32_t t = threadIdx.x & (tpr - 1);                       // thread of the row
+  const uint32_t sub_row = threadIdx.x / tpr, per_step = THREADS / tpr;
+  const uint32_t groups = (p.cols8 + 15) >> 4, row_slots = (tpr >> 4) * VEC;
   uint4* const mine = places + threadIdx.x;
   const uint32_t mine_at = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
   HB_LAUNCH_DEPENDENTS();
-  auto request = [&](int64_t row, int stage) {
+  auto request = [&](uint32_t row, int stage) {
     if (row < p.rows) {
       const uint4* xr = reinterpret_cast<const uint4*>(p.x + row * p.ldx) + t;
       const uint4* rr = reinterpret_cast<const uint4*>(p.residual + row * p.ldr) + t;
@@ -166,8 +164,8 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int64_t row = static_cast<int64_t>(blockIdx.x) * per_step + sub_row;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * per_step;
+  uint32_t row = blockIdx.x * per_step + sub_row;
+  const uint32_t step = gridDim.x * per_step;
 #pragma unroll
   for (int s = 0; s < L::STAGES; ++s) request(row + s * step, s);
   float2 gain[L::GAIN_IN_REGS ? VEC : 1][4];
@@ -183,9 +181,9 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
     }
   }
   int buf = 0, stage = 0;
-  for (int64_t base = row - sub_row; base < p.rows; base += BATCH * step, buf ^= 1) {   // every thread of the CTA takes every step
+  for (uint32_t base = row - sub_row; base < p.rows; base += BATCH * step, buf ^= 1) {   // every thread of the CTA takes every step
 #pragma unroll 1
-    for (int j = 0; j < BATCH && base + j * step < p.rows; ++j, row += step) {
+    for (uint32_t j = 0; j < BATCH && base + j * step < p.rows; ++j, row += step) {
       asm volatile("cp.async.wait_group %0;" ::"n"(L::STAGES - 1) : "memory");
       const uint4* now = mine + stage * L::PER_STAGE;
       float ss = 0.f;
@@ -226,15 +224,15 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
       }
       request(row + L::STAGES * step, stage);
       if (++stage == L::STAGES) stage = 0;
-      for (int o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      for (uint32_t o = (tpr < 32 ? tpr : 32) / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if ((t & 31) == 0) red[buf][j][tpr < 32 ? sub_row : threadIdx.x >> 5] = ss;
     }
     __syncthreads();                                                // the other buffers are rewritten behind the next one
-    const int j = threadIdx.x / SLOTS, slot = threadIdx.x % SLOTS, sub = slot / row_slots, g = slot % row_slots;
-    const int64_t at = base + j * step + sub;
+    const uint32_t j = threadIdx.x / SLOTS, slot = threadIdx.x % SLOTS, sub = slot / row_slots, g = slot % row_slots;
+    const uint32_t at = base + j * step + sub;
     if (j < BATCH && g < groups && at < p.rows) {
       float ss = 0.f;
-      for (int w = 0; w < warps; ++w) ss += red[buf][j][sub * warps + w];
+      for (uint32_t w = 0; w < warps; ++w) ss += red[buf][j][sub * warps + w];
       const float inv_rms = rsqrtf(ss * p.inv_cols + p.eps), top = tops[buf][j][slot];
       Scale z = finite_scale_of(top * inv_rms);
       if (!(top >= Q_TOP * Q_FLOOR && z.s > Q_FLOOR && z.s < INFINITY) && !(top == 0.f && inv_rms < INFINITY)) {
@@ -243,7 +241,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
         const __nv_bfloat16* gain = reinterpret_cast<const __nv_bfloat16*>(p.gain) + g * QG;
         uint8_t* q = p.q + at * p.ldq + g * QG;
 #pragma unroll 1
-        for (int k = 0; k < min(QG, p.cols8 * 8 - g * QG); ++k)
+        for (uint32_t k = 0; k < min(uint32_t{QG}, p.cols8 * 8 - g * QG); ++k)
           q[k] = __nv_cvt_float_to_fp8(__bfloat162float(v[k]) * __bfloat162float(gain[k]) * inv_rms * z.to_q, __NV_SATFINITE, __NV_E4M3);
       }
       p.scale[at * p.ss0 + g * p.ss1] = z.s;
@@ -258,8 +256,8 @@ struct RowParams {
   const void* x;
   uint8_t* q;
   float* scale;
-  int64_t rows;
-  int64_t ldx, ldq, ss0, ss1;
+  uint32_t rows;
+  uint64_t ldx, ldq, ss0, ss1;
   int cols;                    // columns of q (SwiGLU: half the columns of x)
 };
 
@@ -278,7 +276,7 @@ template <int SRC, bool VEC>
 struct Values {
   uint4 a, b;                  // VEC: the 16-byte vectors (b: the up half, or the second four fp32 values)
   float f[8];                  // otherwise
-  __device__ __forceinline__ void load(const RowParams& p, int64_t row, int c) {
+  __device__ __forceinline__ void load(const RowParams& p, uint32_t row, int c) {
     if constexpr (SRC == SRC_SWIGLU) {
       const __nv_bfloat16* base = static_cast<const __nv_bfloat16*>(p.x) + row * p.ldx + c * 8;
       a = *reinterpret_cast<const uint4*>(base);
@@ -332,7 +330,7 @@ struct Values {
 };
 
 template <bool VEC>
-__device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, const float (&y)[8], const Scale& z) {
+__device__ __forceinline__ void store8(const RowParams& p, uint32_t row, int c, const float (&y)[8], const Scale& z) {
   uint8_t* dst = p.q + row * p.ldq;
   const uint2 w = pack8(y, z);
   if constexpr (VEC) {
@@ -345,13 +343,15 @@ __device__ __forceinline__ void store8(const RowParams& p, int64_t row, int c, c
 }
 
 // blockDim = (columns / 8 covered at once, rows): every run of 16 threads in x is one group.  A thread takes
-// the same columns of UNROLL rows, all of them requested before the first is used: with one 16-byte load
-// per thread 8192 x 4096 bf16 took 21.7 us, with four 19.2 (5.3 TB/s); fp32 27 us (6.2 TB/s); SwiGLU
-// 8192 x 14336 100 us (5.9 TB/s).  Rows that allow no 16-byte vectors (8192 x 4001): 28 us.
+// the same columns of UNROLL rows, all of them requested before the first is used.  Bound by HBM: with one
+// 16-byte load per thread 8192 x 4096 bf16 took 21.7 us, with two 17.1, three 16.4 (6.2 TB/s), four 18.7, eight
+// 19.1; fp32 26.0 us with three (6.5 TB/s); SwiGLU 8192 x 14336 94 us (6.2 TB/s).  Rows that allow no 16-byte
+// vectors (8192 x 4001): 25.7 us.
+constexpr int ROWS_MANY = 3;
 template <int SRC, bool VEC, int UNROLL>
 __global__ void __launch_bounds__(256) quant_rows_kernel(const RowParams p) {
   HB_LAUNCH_DEPENDENTS();
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * blockDim.y * UNROLL + threadIdx.y;
+  const uint32_t row0 = blockIdx.x * blockDim.y * UNROLL + threadIdx.y;
   const int c = blockIdx.y * blockDim.x + threadIdx.x;
   const bool mine = (VEC ? c * 8 : loose_col(c, 0)) < p.cols;
   const int c_load = mine ? c : 0;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const RowParams p) {
   for (int i = 0; i < UNROLL; ++i) v[i].load(p, min(row0 + i * blockDim.y, p.rows - 1), c_load);
 #pragma unroll
   for (int i = 0; i < UNROLL; ++i) {
-    const int64_t row = row0 + i * blockDim.y;
+    const uint32_t row = row0 + i * blockDim.y;
     float y[8];
     v[i].widen(y);
     const Scale z = scale_of(group_max(mine ? abs_max8(y) : 0.f));
@@ -373,13 +373,13 @@ __global__ void __launch_bounds__(256) quant_rows_kernel(const RowParams p) {
 
 // ------------------------------------------------------------------ 128 x 128 blocks
 // One CTA per block, 64 values per thread in registers: 16 threads span the 128 columns, 16 rows
-// are read at a time.  Bound by HBM: 28672 x 4096 from fp32 95 us (6.2 TB/s), from bf16 56 us (6.3 TB/s; 73 us
-// while the values were widened before the maximum and so took twice the registers).
+// are read at a time.  Bound by HBM: 28672 x 4096 from fp32 94 us (6.2 TB/s), from bf16 57 us (6.2 TB/s; 65 us
+// with two CTAs per SM instead of three).
 template <int SRC, bool VEC>
-__global__ void __launch_bounds__(256) quant_blocks_kernel(const RowParams p) {
+__global__ void __launch_bounds__(256, VEC ? 3 : 2) quant_blocks_kernel(const RowParams p) {
   __shared__ float red[8];
   HB_LAUNCH_DEPENDENTS();
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * QG + (threadIdx.x >> 4);
+  const uint32_t row0 = blockIdx.x * QG + (threadIdx.x >> 4);
   const int c = blockIdx.y * (QG / 8) + (threadIdx.x & 15);
   const bool live = (VEC ? c * 8 : loose_col(c, 0)) < p.cols;
   const int c_load = live ? c : 0;
@@ -449,10 +449,10 @@ hb_status launch_rows(hb_ctx* ctx, const RowParams& p, const char* what) {
   const int64_t across = (vecs + tx - 1) / tx;
   if (across > 65535) return hb_fail(ctx, HB_ERR_UNSUPPORTED, "%s: too many columns", what);
   // several rows per thread once there is work for every SM with that
-  const bool many = (p.rows + 4 * ty - 1) / (4 * ty) * across >= 4 * ctx->sm_count;
-  const int rows = many ? 4 * ty : ty;
+  const bool many = (p.rows + ROWS_MANY * ty - 1) / (ROWS_MANY * ty) * across >= 4 * ctx->sm_count;
+  const int rows = many ? ROWS_MANY * ty : ty;
   const dim3 grid((unsigned)((p.rows + rows - 1) / rows), (unsigned)across);
-  const cudaError_t e = hb_launch_dependent(many ? quant_rows_kernel<SRC, VEC, 4> : quant_rows_kernel<SRC, VEC, 1>, grid, dim3(tx, ty),
+  const cudaError_t e = hb_launch_dependent(many ? quant_rows_kernel<SRC, VEC, ROWS_MANY> : quant_rows_kernel<SRC, VEC, 1>, grid, dim3(tx, ty),
                                             0, ctx->stream, p);
   if (e != cudaSuccess) { cudaGetLastError(); return hb_check_cuda(ctx, e, what); }
   ctx->launches++;
@@ -479,8 +479,8 @@ hb_status quantize(hb_ctx* ctx, const hb_tensor* x, hb_tensor* q, hb_tensor* sca
   if ((st = check_pair(ctx, op, q, scale, rows, cols, block_rows)) != HB_OK) return st;
   const int es = x->dtype == HB_BF16 ? 2 : 4;
   if (reinterpret_cast<uintptr_t>(x->ptr) & (es - 1)) return hb_fail(ctx, HB_ERR_INVALID, "%s: misaligned pointer", op);
-  RowParams p = {x->ptr, static_cast<uint8_t*>(q->ptr), static_cast<float*>(scale->ptr), rows, x->stride[0], q->stride[0],
-                 scale->stride[0], scale->stride[1], (int)cols};
+  RowParams p = {x->ptr, static_cast<uint8_t*>(q->ptr), static_cast<float*>(scale->ptr), (uint32_t)rows, (uint64_t)x->stride[0], (uint64_t)q->stride[0],
+                 (uint64_t)scale->stride[0], (uint64_t)scale->stride[1], (int)cols};
   // whole 16-byte vectors wherever every row starts on one and ends on one
   const bool vec = cols % 8 == 0 && aligned(x->ptr, x->stride[0] * es, 16) && aligned(q->ptr, q->stride[0], 8);
   hb_device_guard guard(ctx);
@@ -502,8 +502,8 @@ hb_status swiglu_quant(hb_ctx* ctx, const hb_tensor* x, hb_tensor* q, hb_tensor*
   if ((st = check_pair(ctx, op, q, scale, rows, half, 1)) != HB_OK) return st;
   if (!aligned(x->ptr, x->stride[0] * 2, 16) || !aligned(q->ptr, q->stride[0], 8))
     return hb_fail(ctx, HB_ERR_INVALID, "%s: rows of x must be 16-byte aligned and rows of the output 8-byte aligned", op);
-  RowParams p = {x->ptr, static_cast<uint8_t*>(q->ptr), static_cast<float*>(scale->ptr), rows, x->stride[0], q->stride[0],
-                 scale->stride[0], scale->stride[1], (int)half};
+  RowParams p = {x->ptr, static_cast<uint8_t*>(q->ptr), static_cast<float*>(scale->ptr), (uint32_t)rows, (uint64_t)x->stride[0], (uint64_t)q->stride[0],
+                 (uint64_t)scale->stride[0], (uint64_t)scale->stride[1], (int)half};
   hb_device_guard guard(ctx);
   return launch_rows<SRC_SWIGLU, true>(ctx, p, op);
 }
@@ -531,8 +531,9 @@ hb_status rmsnorm_quant(hb_ctx* ctx, const hb_tensor* x, const void* gain, hb_te
   const int threads = tpr > 256 ? tpr : 256;
   NormParams p = {static_cast<const __nv_bfloat16*>(x->ptr), static_cast<const uint4*>(gain),
                   res ? static_cast<__nv_bfloat16*>(res->ptr) : nullptr, static_cast<uint8_t*>(q->ptr),
-                  static_cast<float*>(scale->ptr), rows, x->stride[0], res ? res->stride[0] : 0, q->stride[0], scale->stride[0],
-                  scale->stride[1], cols8, tpr, 1.0f / (float)cols, eps};
+                  static_cast<float*>(scale->ptr), (uint32_t)rows, (uint64_t)x->stride[0], (uint64_t)(res ? res->stride[0] : 0),
+                  (uint64_t)q->stride[0], (uint64_t)scale->stride[0], (uint64_t)scale->stride[1], (uint32_t)cols8, (uint32_t)tpr,
+                  1.0f / (float)cols, eps};
   hb_device_guard guard(ctx);
   int variant, bytes;
   void (*kern)(NormParams);
