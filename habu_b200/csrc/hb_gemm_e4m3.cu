@@ -543,14 +543,13 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
         if (!mbar_wait(bar_tfull + slot * 8, slot_phase, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const uint32_t t = t_mine + slot * BN;
-        uint32_t v[2][16];
-        tmem_ld_32x16(t, v[0]);
+        // sixty-four columns at a time: the other warp of the scheduler adds while this one's are on their way
+        uint32_t v[64];
 #pragma unroll
-        for (int c = 0; c < HALF / 16; ++c) {
+        for (int c = 0; c < HALF / 64; ++c) {
+          tmem_ld_32x64(t + c * 64, v);
           tmem_wait_ld();
-          if (c + 1 < HALF / 16) {
-            tmem_ld_32x16(t + (c + 1) * 16, v[(c + 1) & 1]);
-          } else {                                   // everything is in registers: the slot is free
+          if (c + 1 == HALF / 64) {                  // everything is in registers: the slot is free
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -559,7 +558,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
             }
           }
 #pragma unroll
-          for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], v[c & 1][2 * j], v[c & 1][2 * j + 1], f);
+          for (int j = 0; j < 32; ++j) fma2(acc[c * 32 + j], v[2 * j], v[2 * j + 1], f);
         }
         if (++slot == L::SLOTS) { slot = 0; slot_phase ^= 1; }
       }
