@@ -16,9 +16,18 @@
 // what the launch holds).
 // Algorithmic traffic per launch: M*K + N*K + 2*M*N bytes and the scales; work 2*M*N*K flop at the
 // 8-bit tensor rate (twice that of bf16).
+//
+// What bounds a large product is the board's power limit, which settles the clock at 1.25 to 1.5 GHz, and
+// at that clock the way of a slot from the tensor cores through the sums and back: a k-block of the
+// 256 x 256 tile takes about 750 clocks, its MMAs 512.  8192 x 4096 x 14336: 400 us in a burst, 467 sustained
+// (2.06 PFLOP/s); 8192 x 28672 x 4096 with SwiGLU 947 us sustained; the same with one scale for all of A and
+// one for B, in a library, 378 and 781 us sustained.  Measured and not taken: slots of 128 columns (each MMA
+// then reads A again: 535 us where this took 509), two buffers of 32 columns behind each other (they do not
+// fit the registers: 560), sums of sixteen columns at a time (472).
 #include <math.h>
 #include <string.h>
 
+#include <atomic>
 #include <new>
 
 #include "hb_internal.h"
@@ -567,7 +576,7 @@ __device__ __forceinline__ void scaled_tile_body(const CUtensorMap& tmA, const C
       const int row0 = tm * L::BM + rank * 128 + q * 32, col0 = tn * BN + h * HALF;
       if (tile + num_units < num_tiles) first_scales(tile + num_units);   // arrive under this tile's output
       if constexpr (SPLIT) {
-        // The CTAs add their sums up: a warp's columns go, sixteen at a time, to the CTA that writes them,
+            // The CTAs add their sums up: a warp's columns go, sixteen at a time, to the CTA that writes them,
         // into its ring -- which is free once its own last k-block is done (xready) -- and are added
         // there in k order.  Warp w of a CTA deals with warps w alone.
         static_assert(HALF == 64, "four pieces of sixteen columns");
@@ -675,8 +684,8 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
   else kern = hb_matmul_scaled_kernel<BN, STAGES, EPI>;
   // persistent CTAs (or pairs) that can run at once; of pairs the occupancy query knows, because not
   // every SM has a neighbour to pair with
-  static int resident[64] = {};
-  if (!resident[ctx->device & 63]) {
+  static std::atomic<int> resident[64];
+  if (!resident[ctx->device & 63].load(std::memory_order_acquire)) {
     HB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN_BYTES));
     int n = ctx->sm_count;
     if constexpr (PAIR) {
@@ -748,6 +757,11 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // practice, and there is no scratch and no counter in global memory that launches could share.
 // With HB_MATMUL_WEIGHTS_B a CTA fills its ring with B before the kernel in front has finished
 // (programmatic dependent launch); what depends on that kernel comes after the wait.
+// 16 x 28672 x 4096 24.0 us, 16 x 128256 x 4096 80.7 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 9.0 us,
+// 64 x 28672 x 4096 31.7 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
+// launch are not it (start, the first bytes, the last sums; a second CTA on the SM would cover them, but
+// of kernels that allocate tensor memory the occupancy query admits one).  Measured and not taken: equal
+// units for all CTAs and partial sums in global memory (28 us for 16 x 28672 x 4096).
 // ------------------------------------------------------------------------------------
 constexpr int FEW_MAX_M = 64;
 constexpr int FEW_THREADS = 224;                 // TMA, MMA, four warps of sums, factors
@@ -1088,9 +1102,9 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   // clusters of S CTAs that can run at once, one CTA per SM
-  static int resident[64][L::MAX_CLUSTER + 1] = {};
-  int* most = resident[ctx->device & 63];
-  if (!most[1]) {
+  static std::atomic<int> resident[64][L::MAX_CLUSTER + 1];       // (that of one CTA is set last)
+  std::atomic<int>* most = resident[ctx->device & 63];
+  if (!most[1].load(std::memory_order_acquire)) {
     HB_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::DYN_BYTES));
     for (int c = L::MAX_CLUSTER; c >= 1; --c) {
       attr[0].val.clusterDim.x = c;
@@ -1098,8 +1112,8 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
       cfg.numAttrs = 1;
       int n = 0;
       if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) { cudaGetLastError(); n = 0; }
-      most[c] = n < ctx->sm_count / c ? n : ctx->sm_count / c;
-      if (c == 1 && most[c] < 1) most[c] = ctx->sm_count;
+      n = n < ctx->sm_count / c ? n : ctx->sm_count / c;
+      most[c].store(c == 1 && n < 1 ? ctx->sm_count : n, std::memory_order_release);
     }
   }
   CUtensorMap tmA, tmB;
@@ -1124,11 +1138,11 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
   double best = 0;
   for (int c = 1; c <= L::MAX_CLUSTER && c <= p.num_kb; ++c) {
     if (most[c] < 1) continue;
-    const int64_t clusters = p.slabs < most[c] ? p.slabs : most[c];
+    const int64_t at_once = most[c], clusters = p.slabs < at_once ? p.slabs : at_once;
     const double cost = (double)((p.slabs + clusters - 1) / clusters) * p.num_kb / c;
     if (p.cluster == 0 || cost < best) { best = cost; p.cluster = c; }
   }
-  const int clusters = p.slabs < most[p.cluster] ? p.slabs : most[p.cluster];
+  const int at_once = most[p.cluster], clusters = p.slabs < at_once ? p.slabs : at_once;
   attr[0].val.clusterDim.x = p.cluster;
   cfg.gridDim = dim3((unsigned)(clusters * p.cluster));
   cfg.numAttrs = g.b_is_weights ? 2 : 1;

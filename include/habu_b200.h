@@ -251,8 +251,8 @@ hb_status hb_argmax(hb_ctx* ctx, const void* x, int32_t* out, int64_t rows, int6
  *                      16-byte aligned bases and row pitches that are multiples of 16; M, N and K
  *                      are free.  `opts` as for hb_matmul (epilogues and HB_MATMUL_WEIGHTS_B;
  *                      config_id must be -1); a residual must not overlap C.
- * The product of few rows keeps fp32 partial sums in context scratch of a fixed size: calls of
- * one context on different streams must be ordered by the caller, as for hb_matmul. */
+ * None of them uses scratch or counters in device memory, and each adds up in a fixed order: equal
+ * inputs give equal bits, and calls may overlap on the GPU. */
 hb_status hb_quantize(hb_ctx* ctx, const hb_tensor* x, hb_tensor* q, hb_tensor* scale, int32_t block_rows);
 hb_status hb_rmsnorm_quant(hb_ctx* ctx, const hb_tensor* x, const void* gain, hb_tensor* q, hb_tensor* scale,
                            hb_tensor* residual_inout, float eps);
