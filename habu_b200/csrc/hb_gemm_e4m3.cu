@@ -757,8 +757,8 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // practice, and there is no scratch and no counter in global memory that launches could share.
 // With HB_MATMUL_WEIGHTS_B a CTA fills its ring with B before the kernel in front has finished
 // (programmatic dependent launch); what depends on that kernel comes after the wait.
-// 16 x 28672 x 4096 24.0 us, 16 x 128256 x 4096 80.7 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 9.0 us,
-// 64 x 28672 x 4096 31.7 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
+// 16 x 28672 x 4096 24.0 us, 16 x 128256 x 4096 80.7 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 8.7 us,
+// 64 x 28672 x 4096 31.6 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
 // launch are not it (start, the first bytes, the last sums; a second CTA on the SM would cover them, but
 // of kernels that allocate tensor memory the occupancy query admits one).  Measured and not taken: equal
 // units for all CTAs and partial sums in global memory (28 us for 16 x 28672 x 4096).
@@ -838,76 +838,83 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
   const int64_t last_start = (u_end - 1) / p.num_kb * p.num_kb;
   const int senders = last_start >= u_begin ? owner_of(last_start + p.num_kb - 1) - rank : 0;
 
-  if (threadIdx.x == 0) {
-    *abort_flag = 0;
-    for (int s = 0; s < L::STAGES; ++s) {
-      mbar_init(bar_full + s * 8, 1);
-      mbar_init(bar_empty + s * 8, 1);
+  // units that fill the ring, and the loader warp's next unit
+  const int fill = static_cast<int>(min(units, static_cast<int64_t>(L::STAGES)));
+  int load_slab = slab0, load_kb = kb0;
+  auto next_load = [&] {
+    if (++load_kb == p.num_kb) { load_kb = 0; load_slab += step; }
+  };
+  if (warp == 0) {
+    if (elect_one()) {
+      tma_prefetch_desc(&tmB);
+      tma_prefetch_desc(&tmA);
+      *abort_flag = 0;
+      for (int s = 0; s < L::STAGES; ++s) {
+        mbar_init(bar_full + s * 8, 1);
+        mbar_init(bar_empty + s * 8, 1);
+      }
+      for (int a = 0; a < FEW_SLOTS; ++a) {
+        mbar_init(bar_tfull + a * 8, 1);
+        mbar_init(bar_tempty + a * 8, 4);
+        mbar_init(bar_ffull + a * 8, 1);
+      }
+      for (int w = 0; w < 4; ++w) mbar_init(bar_xfull + w * 8, max(senders, 1));
+      mbar_fence_init();
+      fence_proxy_async_smem();
     }
-    for (int a = 0; a < FEW_SLOTS; ++a) {
-      mbar_init(bar_tfull + a * 8, 1);
-      mbar_init(bar_tempty + a * 8, 4);
-      mbar_init(bar_ffull + a * 8, 1);
+    __syncwarp();
+    cluster_arrive();           // the partners may use these barriers
+    // ring fill: B at once -- it needs neither the cluster nor tensor memory nor, being weights, the kernel in
+    // front; A comes from the MMA warp, so that it does not queue behind all of B.  (After the cluster's barrier
+    // and with A behind it 1 x 4096 x 4096 took 7.05 us, so it takes 6.73.)
+    for (int i = 0; i < fill; ++i) {
+      if (elect_one()) {
+        mbar_arrive_expect_tx(bar_full + i * 8, L::A_BYTES + L::B_BYTES);
+        tma_load_2d(sB + i * L::B_BYTES, &tmB, bar_full + i * 8, load_kb * KB, load_slab * SLAB);
+      }
+      next_load();
     }
-    for (int w = 0; w < 4; ++w) mbar_init(bar_xfull + w * 8, max(senders, 1));
-    mbar_fence_init();
-    fence_proxy_async_smem();
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    __syncwarp();
+    cluster_wait();
   }
   if (warp == 1) {
     tmem_alloc<1>(smem_u32(const_cast<uint32_t*>(tmem_ptr_smem)), L::TMEM_COLS);
     tmem_relinquish<1>();
   }
-  tc_fence_before();
-  cluster_sync();               // the partners' barriers are initialised
-  tc_fence_after();
+  if (warp != 0) {
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+  }
   const uint32_t tmem_base = *tmem_ptr_smem;
   grid_launch_dependents();     // the next kernel on the stream may begin its own prologue
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     bool ok = true;
-    // ring fill: B before the dependency wait, A after it; the stages are empty at the start
-    const int fill = static_cast<int>(min(units, static_cast<int64_t>(L::STAGES)));
-    int slab = slab0, kb = kb0;
-    auto next = [&] {
-      if (++kb == p.num_kb) { kb = 0; slab += step; }
-    };
-    for (int i = 0; i < fill; ++i) {
-      if (elect_one()) {
-        mbar_arrive_expect_tx(bar_full + i * 8, L::A_BYTES + L::B_BYTES);
-        tma_load_2d(sB + i * L::B_BYTES, &tmB, bar_full + i * 8, kb * KB, slab * SLAB);
-      }
-      __syncwarp();
-      next();
-    }
-    const int slab_behind = slab, kb_behind = kb;
     grid_dependency_wait();
-    kb = kb0;
-    for (int i = 0; i < fill; ++i) {
-      if (elect_one()) tma_load_2d(sA + i * L::A_BYTES, &tmA, bar_full + i * 8, kb * KB, 0);
-      __syncwarp();
-      next();
-    }
-    slab = slab_behind;
-    kb = kb_behind;
     int s = fill == L::STAGES ? 0 : fill;
     uint32_t phase = fill == L::STAGES ? 1 : 0;
     for (int64_t u = fill; u < units; ++u) {
       if (!mbar_wait(bar_empty + s * 8, phase ^ 1, abort_flag)) { ok = false; break; }
       if (elect_one()) {
         mbar_arrive_expect_tx(bar_full + s * 8, L::A_BYTES + L::B_BYTES);
-        tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, kb * KB, slab * SLAB);
-        tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, kb * KB, 0);
+        tma_load_2d(sB + s * L::B_BYTES, &tmB, bar_full + s * 8, load_kb * KB, load_slab * SLAB);
+        tma_load_2d(sA + s * L::A_BYTES, &tmA, bar_full + s * 8, load_kb * KB, 0);
       }
       __syncwarp();
-      next();
+      next_load();
       if (++s == L::STAGES) { s = 0; phase ^= 1; }
     }
     if (!ok && lane == 0) report_timeout(p.status, 11);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA issuer
+    grid_dependency_wait();
+    for (int i = 0, kb = kb0; i < fill; ++i) {
+      if (elect_one()) tma_load_2d(sA + i * L::A_BYTES, &tmA, bar_full + i * 8, kb * KB, 0);
+      if (++kb == p.num_kb) kb = 0;
+    }
+    __syncwarp();
     constexpr uint32_t idesc = umma_idesc_e4m3(SLAB, MP);
     const uint32_t a_lo = desc_lo(sA), b_lo = desc_lo(sB);
     int s = 0, slot = 0;
