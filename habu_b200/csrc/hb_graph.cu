@@ -210,6 +210,11 @@ extern "C" hb_status hb_graph_add(hb_graph* g, const hb_node* n) {
       return hb_fail(g->ctx, HB_ERR_NOT_FOUND, "graph: %s node optional input %d names unknown tensor %d", kNodeNames[n->kind], i, n->in[i]);
   }
   if (!valid_id(g, n->out)) return hb_fail(g->ctx, HB_ERR_NOT_FOUND, "graph: %s node output names unknown tensor %d", kNodeNames[n->kind], n->out);
+  // The other nodes hand bare pointers on and take their elements for two bytes or four.
+  if (n->kind < HB_NODE_QUANTIZE)
+    for (int id : {n->in[0], n->in[1], n->in[2], n->in[3], n->out})
+      if (id >= 0 && g->tensors[id].dtype == HB_E4M3)
+        return hb_fail(g->ctx, HB_ERR_UNSUPPORTED, "graph: a %s node takes no e4m3 tensor", kNodeNames[n->kind]);
   if (n->kind == HB_NODE_MATMUL_SCALED && (n->iparam[0] & 0xff) == HB_EPI_RESIDUAL)
     return hb_fail(g->ctx, HB_ERR_UNSUPPORTED, "graph: a matmul_scaled node has no residual input");
   // Only the collective nodes may run on the side stream.  The executor orders nodes on

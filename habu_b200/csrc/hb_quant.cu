@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
   float2 gain[L::GAIN_IN_REGS ? VEC : 1][4];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const uint4 g = __ldg(p.gain + min(t + i * tpr, p.cols8 - 1));
+    const uint4 g = p.gain[min(t + i * tpr, p.cols8 - 1)];   // (a plain load: the kernel in front may have written it)
     if constexpr (L::GAIN_IN_REGS) {
       const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll

@@ -65,6 +65,13 @@ class Tensor:
         return self._c[1]
 
 
+def _plain(*tensors: Optional[Tensor]):
+    """Refuses e4m3 tensors where an operator takes bare pointers to wider elements."""
+    for t in tensors:
+        if t is not None and t.dtype == HB_E4M3:
+            raise HabuError(_capi.HB_ERR_UNSUPPORTED, "only the operators of the 8-bit path take e4m3 tensors")
+
+
 def f32_to_bf16_bits(x: np.ndarray) -> np.ndarray:
     """Host-side fp32 -> bf16 bit patterns, round to nearest even (NaNs stay NaNs)."""
     u = np.ascontiguousarray(x, np.float32).view(np.uint32)
@@ -216,12 +223,14 @@ class Context:
                     base: float = 10000.0):
         """RoPE of the new token's q and k heads at position pos[0] (in place in `qkv`
         [batch, row]) and append of k and v to `kv_cache` [2*batch, s_max, kv_heads, 128]."""
+        _plain(qkv, kv_cache, pos)
         self._check(_lib.hb_rope_append(self._h, qkv.ptr, qkv.stride[0], kv_cache.ptr, pos.ptr, qkv.shape[0], n_q_heads,
                                         n_kv_heads, kv_cache.shape[3], kv_cache.shape[1], base))
 
     def attention_decode(self, qkv: Tensor, kv_cache: Tensor, pos: Tensor, n_q_heads: int, n_kv_heads: int,
                          out: Optional[Tensor] = None, scale: Optional[float] = None, len_hint: int = 0) -> Tensor:
         """Single-query attention of each sequence's new token over cache positions 0..pos[0]."""
+        _plain(qkv, kv_cache, pos, out)
         D = kv_cache.shape[3]
         if out is None:
             out = self.empty((qkv.shape[0], n_q_heads * D))
@@ -237,6 +246,7 @@ class Context:
     # -- glue ---------------------------------------------------------------------
     def rmsnorm(self, x: Tensor, gain: Tensor, out: Optional[Tensor] = None, eps: float = 1e-5,
                 residual: Optional[Tensor] = None) -> Tensor:
+        _plain(x, gain, out, residual)
         rows, cols = x.shape
         if out is None:
             out = self.empty(x.shape, x.dtype)
@@ -245,11 +255,13 @@ class Context:
         return out
 
     def rope(self, x: Tensor, seq: int, heads: int, head_dim: int, base: float = 10000.0, pos0: int = 0) -> Tensor:
+        _plain(x)
         tokens = x.shape[0]
         self._check(_lib.hb_rope(self._h, x.ptr, tokens, seq, heads, head_dim, x.stride[0], base, pos0))
         return x
 
     def embedding(self, table: Tensor, ids: Tensor, out: Optional[Tensor] = None) -> Tensor:
+        _plain(table, ids, out)
         tokens = ids.shape[0]
         vocab, dim = table.shape
         if out is None:
@@ -258,6 +270,7 @@ class Context:
         return out
 
     def swiglu(self, x: Tensor, out: Optional[Tensor] = None) -> Tensor:
+        _plain(x, out)
         rows, two = x.shape
         if out is None:
             out = self.empty((rows, two // 2), x.dtype)
@@ -265,18 +278,21 @@ class Context:
         return out
 
     def gelu(self, x: Tensor, out: Optional[Tensor] = None) -> Tensor:
+        _plain(x, out)
         if out is None:
             out = self.empty(x.shape, x.dtype)
         self._check(_lib.hb_gelu(self._h, x.ptr, out.ptr, x.nbytes // 2))
         return out
 
     def gelu_backward(self, x: Tensor, dy: Tensor, out: Optional[Tensor] = None) -> Tensor:
+        _plain(x, dy, out)
         if out is None:
             out = self.empty(x.shape, x.dtype)
         self._check(_lib.hb_gelu_backward(self._h, x.ptr, dy.ptr, out.ptr, x.nbytes // 2))
         return out
 
     def add(self, a: Tensor, b: Tensor, out: Optional[Tensor] = None) -> Tensor:
+        _plain(a, b, out)
         if out is None:
             out = self.empty(a.shape, a.dtype)
         self._check(_lib.hb_add(self._h, a.ptr, b.ptr, out.ptr, a.nbytes // 2))
@@ -284,6 +300,7 @@ class Context:
 
     def mse(self, y: Tensor, target: Tensor, dy: Optional[Tensor] = None, loss: Optional[Tensor] = None):
         """Returns (loss tensor f32[1], dy) for mean((y - target)^2)."""
+        _plain(y, target, dy, loss)
         if dy is None:
             dy = self.empty(y.shape, y.dtype)
         if loss is None:
@@ -300,6 +317,7 @@ class Context:
                        grad_scale))
 
     def argmax(self, x: Tensor) -> Tensor:
+        _plain(x)
         rows, cols = x.shape
         out = self.empty((rows,), HB_I32)
         self._check(_lib.hb_argmax(self._h, x.ptr, out.ptr, rows, cols))
@@ -309,16 +327,21 @@ class Context:
     def empty_quantised(self, rows: int, cols: int, block_rows: int = 1):
         """A (q, scale) pair for [rows, cols]: e4m3 rows padded to a multiple of 16 bytes (what
         the scaled product loads) and one fp32 scale per 128 values or 128 x 128 block."""
-        q = self.empty((rows, (cols + 15) // 16 * 16), HB_E4M3)
-        q.shape = (rows, cols)
-        return q, self.empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), HB_F32)
+        return self._pair(None, None, rows, cols, block_rows)
+
+    def _pair(self, q: Optional[Tensor], scale: Optional[Tensor], rows: int, cols: int, block_rows: int = 1):
+        """(q, scale) with what is missing allocated."""
+        if q is None:
+            q = self.empty((rows, (cols + 15) // 16 * 16), HB_E4M3)
+            q.shape = (rows, cols)
+        if scale is None:
+            scale = self.empty(((rows + block_rows - 1) // block_rows, (cols + 127) // 128), HB_F32)
+        return q, scale
 
     def quantize(self, x: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None, block_rows: int = 1):
         """x [rows, cols] bf16 or fp32 -> (q e4m3 [rows, cols], scale fp32): one scale per 128
         values of a row (block_rows=1) or per 128 x 128 block (block_rows=128, weights)."""
-        if out is None or scale is None:
-            q, s = self.empty_quantised(*x.shape, block_rows)
-            out, scale = out or q, scale or s
+        out, scale = self._pair(out, scale, *x.shape, block_rows)
         tx, tq, ts = x.c(), out.c(), scale.c()
         self._check(_lib.hb_quantize(self._h, C.byref(tx), C.byref(tq), C.byref(ts), block_rows))
         return out, scale
@@ -326,9 +349,7 @@ class Context:
     def rmsnorm_quant(self, x: Tensor, gain: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None,
                       eps: float = 1e-5, residual: Optional[Tensor] = None):
         """RMSNorm (after residual += x in place, if given) quantised to (q, scale)."""
-        if out is None or scale is None:
-            q, s = self.empty_quantised(*x.shape)
-            out, scale = out or q, scale or s
+        out, scale = self._pair(out, scale, *x.shape)
         tx, tq, ts = x.c(), out.c(), scale.c()
         tr = C.byref(residual.c()) if residual is not None else None
         self._check(_lib.hb_rmsnorm_quant(self._h, C.byref(tx), gain.ptr, C.byref(tq), C.byref(ts), tr, eps))
@@ -336,9 +357,7 @@ class Context:
 
     def swiglu_quant(self, x: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None):
         """silu(x[:, :half]) * x[:, half:] quantised to (q, scale)."""
-        if out is None or scale is None:
-            q, s = self.empty_quantised(x.shape[0], x.shape[1] // 2)
-            out, scale = out or q, scale or s
+        out, scale = self._pair(out, scale, x.shape[0], x.shape[1] // 2)
         tx, tq, ts = x.c(), out.c(), scale.c()
         self._check(_lib.hb_swiglu_quant(self._h, C.byref(tx), C.byref(tq), C.byref(ts)))
         return out, scale

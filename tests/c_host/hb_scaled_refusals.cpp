@@ -135,6 +135,25 @@ int main() {
   mm("residual misaligned", [&](M& a) { a.o.epilogue = HB_EPI_RESIDUAL; a.o.residual = P + 1; }, INV, "misaligned");
   expect(ctx, "null tensors", hb_matmul_scaled(&ctx, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr), INV, "null");
   if (hb_matmul_scaled(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr) != INV) { puts("null context accepted"); ++bad; }
+
+  // ---- graph: every other node takes its tensors' elements for two bytes or four
+  hb_graph* g = nullptr;
+  if (hb_graph_create(&ctx, &g) != HB_OK) { puts("no graph"); return 1; }
+  const hb_tensor q = mat(P, HB_E4M3, 64, 256, 256, 1), w = mat(P, HB_BF16, 64, 256, 256, 1);
+  int32_t iq = -1, iw = -1;
+  hb_graph_input(g, &q, &iq);
+  hb_graph_input(g, &w, &iw);
+  for (int kind = HB_NODE_MATMUL; kind < HB_NODE_QUANTIZE; ++kind)
+    for (int at = 0; at < 5; ++at) {
+      hb_node n;
+      memset(&n, 0, sizeof(n));
+      n.kind = kind;
+      for (int i = 0; i < 4; ++i) n.in[i] = at == i ? iq : iw;
+      n.out = at == 4 ? iq : iw;
+      ctx.err.clear();
+      expect(ctx, "e4m3 in another node", hb_graph_add(g, &n), UNS, "e4m3");
+    }
+  hb_graph_destroy(g);
   if (ctx.launches) { puts("something was launched"); ++bad; }
   return bad ? 1 : 0;
 }

@@ -194,3 +194,16 @@ def test_decoder_graph_refuses_what_e4m3_does_not_cover(ctx):
     one = DecoderGraph(ctx, CFG, 1, 0, layers)
     with pytest.raises(ValueError, match="same precision"):
         DecoderGraph(ctx, CFG, 1, 0, layers, e4m3=True, share=one)
+
+
+def test_other_operators_refuse_e4m3(ctx):
+    """An e4m3 tensor where an operator takes bare pointers to wider elements is refused before a launch."""
+    q, _ = ctx.quantize(ctx.upload(np.zeros((32, 256), np.uint16)))
+    gain, ids = ctx.upload(np.zeros(256, np.uint16)), ctx.upload(np.zeros(4, np.int32))
+    before = ctx.launches
+    for call in (lambda: ctx.rmsnorm(q, gain), lambda: ctx.rmsnorm(gain, gain, out=q), lambda: ctx.rope(q, 32, 2, 128), lambda: ctx.embedding(q, ids),
+                 lambda: ctx.swiglu(q), lambda: ctx.gelu(q), lambda: ctx.add(q, q), lambda: ctx.argmax(q), lambda: ctx.mse(q, q),
+                 lambda: ctx.matmul(q, q.T)):
+        with pytest.raises(hb.HabuError):
+            call()
+    assert ctx.launches == before
