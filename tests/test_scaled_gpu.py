@@ -1,6 +1,7 @@
 """8-bit path: quantisation to e4m3 with a scale per 128 values (plain, behind RMSNorm and behind
 SwiGLU) and the block-scaled product, against 64-bit restatements (tests/quant_ref.py)."""
 import ctypes as C
+import math
 
 import numpy as np
 import pytest
@@ -591,3 +592,42 @@ def test_rmsnorm_quant_around_the_floor(ctx, rows, cols, residual):
     # rows of unit variance) and a scale of 2^-126 or more turn into 1.2 * 2^-24 units of q
     good = [0] + list(range(4, rows))
     qr.check_pair(qr.rmsnorm(x[good], g, 1e-5), q[good], s[good], 1, 2.0 ** -17, 2.0 ** -23)
+
+
+@pytest.mark.parametrize("step,K", [(64, 16), (1, 256), (100, 4096), (1300, 16)])
+def test_gelu_epilogue_over_its_range(ctx, step, K):
+    """Products of a single 1 with a_scale as the argument: from far below zero, where the output is a
+    vanishing product, through zero to far above, infinities and NaN; every form of the product."""
+    x = np.concatenate([np.linspace(-14, 14, 700), np.linspace(-6, 6, 500), [0.0, -0.0, 1e-30, -1e-30, 1e30, -1e30, 3e38, -3e38],
+                        np.linspace(-0.01, 0.01, 92)]).astype(np.float32)
+    if step == 1:
+        x = x[::50]
+    N = 24
+    one = np.zeros((step, K), np.uint8)
+    one[:, 3] = qr.encode(np.ones(1))[0]
+    w = np.zeros((N, K), np.uint8)
+    w[:, 3] = one[0, 3]
+    A, B = ctx.upload(one), ctx.upload(w)
+    SB = ctx.upload(np.ones((1, K // 128 if K > 128 else 1), np.float32))
+    got = []
+    for at in range(0, len(x), step):
+        s = np.ones((step, SB.shape[1]), np.float32)
+        part = x[at:at + step]
+        s[:len(part), 0] = part
+        c = ctx.matmul_scaled(A, ctx.upload(s), B.T, SB.T, epilogue=hb.HB_EPI_GELU)
+        got.append(oracle.from_bf16_bits(ctx.download(c))[:len(part)])
+    got = np.concatenate(got).astype(np.float64)
+    v = x.astype(np.float64)
+    tail = np.array([0.5 * abs(t) * math.erfc(abs(t) / math.sqrt(2)) for t in v])
+    want = np.maximum(v, 0) - tail
+    # erfc to 2^-17 of itself (|x| < 5.2), 2^-14 (up to 6), 2^-4.9; three roundings to fp32; the one to bf16.
+    # The exponential gives 0 for an erfc below 2^-126: the product with |x| / 2 then loses at most
+    # |x| / 2 * 2^-126 (and |x| / 2 is taken as 8 at most).
+    off = np.where(np.abs(v) < 5.2, 2.0 ** -17, np.where(np.abs(v) < 6, 2.0 ** -14, 2.0 ** -4.9))
+    tol = np.abs(want) * (2.0 ** -8 + 2.0 ** -21) + tail * off * (1 + 2.0 ** -8) + np.minimum(np.abs(v) / 2, 8) * 2.0 ** -126 + 2.0 ** -133
+    assert np.all(np.abs(got - want[:, None]) <= tol[:, None])
+    s = np.ones((step, SB.shape[1]), np.float32)
+    for value in (np.inf, np.nan):
+        s[0, 0] = value
+        c = oracle.from_bf16_bits(ctx.download(ctx.matmul_scaled(A, ctx.upload(s), B.T, SB.T, epilogue=hb.HB_EPI_GELU)))
+        assert np.isnan(c[0]).all() if np.isnan(value) else (c[0] == np.inf).all()
