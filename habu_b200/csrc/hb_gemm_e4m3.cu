@@ -149,7 +149,7 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
 // x Phi(x) = max(x, 0) - b erfc(sqrt(2) b) with b = |x| / 2, where nothing cancels.  -log2 erfc(sqrt(2) b) is smooth
 // and nearly a parabola: a polynomial of degree 8 without a constant (least squares, the weights moved
 // towards the largest error) and one exponential give erfc to 2^-17 of itself for |x| < 5.2, 2^-14 up to 6 and 2^-5
-// beyond, where the product is below 1e-8; the rounding to bf16 takes 2^-9.  Two values at a time.  With
+// beyond, where the product is below 1e-8; the rounding to bf16 takes up to 2^-8.  Two values at a time.  With
 // 0.5 x (1 + erff(x / sqrt(2))) 3766 x 22616 x 384 took 163 us, so it takes 96 (59 without an epilogue).
 __device__ __forceinline__ void gelu2(float& x, float& y) {
   constexpr float Q[8] = {-2.30247927f, -1.83368206f, -0.432660699f, 0.137890294f, -0.0313005634f, 0.00462997565f, -0.000390943867f, 1.40522461e-05f};
@@ -250,22 +250,30 @@ __device__ __forceinline__ void move_pieces(const Rows& m, uint32_t buf, int lan
   constexpr int STEPS = 32 / ROWS, BATCH = STEPS < 8 ? STEPS : 8;   // steps whose loads go out together
   const int in_row = lane % PER_ROW * WIDTH, col = col0 + in_row / 2;
   const bool whole = col + WIDTH / 2 <= m.cols;
+  const int left = whole ? m.rows - row0 : 0;                       // rows of the block that exist
+  const char* mem = reinterpret_cast<const char*>(m.base) + (row0 + lane / PER_ROW) * m.pitch + 2 * static_cast<int64_t>(col);
+  const int64_t step = ROWS * m.pitch;
 #pragma unroll 1
   for (int s0 = 0; s0 < STEPS; s0 += BATCH) {
     T v[BATCH] = {};
     const int r0 = s0 * ROWS + lane / PER_ROW;
+    const char* at = mem;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       const int r = r0 + i * ROWS;
       if constexpr (STORE) ld_shared(piece_at<COLS>(buf, r, in_row >> 4) + (in_row & 15), v[i]);
-      else if (whole && row0 + r < m.rows) v[i] = *reinterpret_cast<const T*>(m.base + (row0 + r) * m.pitch + 2 * static_cast<int64_t>(col));
+      else if (r < left) v[i] = *reinterpret_cast<const T*>(at);
+      at += step;
     }
+    at = mem;
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       const int r = r0 + i * ROWS;
       if constexpr (!STORE) st_shared(piece_at<COLS>(buf, r, in_row >> 4) + (in_row & 15), v[i]);
-      else if (whole && row0 + r < m.rows) *reinterpret_cast<T*>(m.base + (row0 + r) * m.pitch + 2 * static_cast<int64_t>(col)) = v[i];
+      else if (r < left) *reinterpret_cast<T*>(const_cast<char*>(at)) = v[i];
+      at += step;
     }
+    mem = at;
   }
   if (WIDTH > 2 && !whole && col < m.cols) {         // the rows end inside this lane's piece
     for (int r = lane / PER_ROW; r < 32 && row0 + r < m.rows; r += ROWS)
