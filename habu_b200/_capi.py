@@ -100,10 +100,11 @@ def load() -> C.CDLL:
         "hb_mse": [vp, vp, vp, vp, vp, i64],
         "hb_adam_step": [vp, vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, i64, f32],
         "hb_adam_step_async": [vp, vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, i64, f32],
-        "hb_quantize": [vp, T, T, T, i32],
-        "hb_rmsnorm_quant": [vp, T, vp, T, T, T, f32],
-        "hb_swiglu_quant": [vp, T, T, T],
-        "hb_matmul_scaled": [vp, T, T, T, T, T, C.POINTER(hb_matmul_opts)],
+        # views by address (Tensor.addr): a typed pointer per argument takes longer to pass than a small launch
+        "hb_quantize": [vp, vp, vp, vp, i32],
+        "hb_rmsnorm_quant": [vp, vp, vp, vp, vp, vp, f32],
+        "hb_swiglu_quant": [vp, vp, vp, vp],
+        "hb_matmul_scaled": [vp, vp, vp, vp, vp, vp, vp],
         "hb_comm_unique_id": [vp],
         "hb_comm_init_rank": [vp, i32, i32, vp],
         "hb_comm_destroy": [vp],

@@ -25,6 +25,7 @@ from ._capi import (HB_AR_AUTO, HB_AR_NCCL, HB_AR_NVLS, HB_AR_P2P, HB_BF16, HB_E
 
 _lib = _capi.load()
 _ELEM = {HB_F32: 4, HB_BF16: 2, HB_I32: 4, HB_E4M3: 1}
+_OPTS = {}          # options of scaled products without a residual, by their epilogue word
 
 
 class HabuError(RuntimeError):
@@ -55,14 +56,22 @@ class Tensor:
         assert len(self.shape) == 2
         return Tensor(self.ptr, self.dtype, self.shape[::-1], self.stride[::-1], self.owner)
 
+    def _view(self) -> tuple:
+        """The fields, the C view made of them and its address.  Making one costs more host time than a
+        small launch, so it is kept until a field is replaced."""
+        k = self._c
+        if k is None or k[0] is not self.ptr or k[1] is not self.dtype or k[2] is not self.shape or k[3] is not self.stride:
+            t = _capi.hb_tensor(self.ptr, self.dtype, len(self.shape), (C.c_int64 * 4)(*self.shape), (C.c_int64 * 4)(*self.stride))
+            k = self._c = (self.ptr, self.dtype, self.shape, self.stride, t, C.addressof(t))
+        return k
+
     def c(self) -> _capi.hb_tensor:
-        """The C view.  Building one costs more host time than a small launch, so it is kept until
-        a field it was made from changes."""
-        key = (self.ptr, self.dtype, self.shape, self.stride)
-        if self._c is None or self._c[0] != key:
-            self._c = key, _capi.hb_tensor(self.ptr, self.dtype, len(self.shape), (C.c_int64 * 4)(*self.shape),
-                                           (C.c_int64 * 4)(*self.stride))
-        return self._c[1]
+        """The C view."""
+        return self._view()[4]
+
+    def addr(self) -> int:
+        """Address of the C view: what entry points declared with plain pointers take."""
+        return self._view()[5]
 
 
 def _plain(*tensors: Optional[Tensor]):
@@ -105,7 +114,7 @@ class Context:
 
     # -- plumbing ---------------------------------------------------------------
     def _check(self, st: int):
-        if st != 0:
+        if st:
             raise HabuError(st, _lib.hb_last_error_string(self._h).decode())
 
     def close(self):
@@ -342,24 +351,21 @@ class Context:
         """x [rows, cols] bf16 or fp32 -> (q e4m3 [rows, cols], scale fp32): one scale per 128
         values of a row (block_rows=1) or per 128 x 128 block (block_rows=128, weights)."""
         out, scale = self._pair(out, scale, *x.shape, block_rows)
-        tx, tq, ts = x.c(), out.c(), scale.c()
-        self._check(_lib.hb_quantize(self._h, C.byref(tx), C.byref(tq), C.byref(ts), block_rows))
+        self._check(_lib.hb_quantize(self._h, x.addr(), out.addr(), scale.addr(), block_rows))
         return out, scale
 
     def rmsnorm_quant(self, x: Tensor, gain: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None,
                       eps: float = 1e-5, residual: Optional[Tensor] = None):
         """RMSNorm (after residual += x in place, if given) quantised to (q, scale)."""
         out, scale = self._pair(out, scale, *x.shape)
-        tx, tq, ts = x.c(), out.c(), scale.c()
-        tr = C.byref(residual.c()) if residual is not None else None
-        self._check(_lib.hb_rmsnorm_quant(self._h, C.byref(tx), gain.ptr, C.byref(tq), C.byref(ts), tr, eps))
+        self._check(_lib.hb_rmsnorm_quant(self._h, x.addr(), gain.ptr, out.addr(), scale.addr(),
+                                          residual.addr() if residual is not None else None, eps))
         return out, scale
 
     def swiglu_quant(self, x: Tensor, out: Optional[Tensor] = None, scale: Optional[Tensor] = None):
         """silu(x[:, :half]) * x[:, half:] quantised to (q, scale)."""
         out, scale = self._pair(out, scale, x.shape[0], x.shape[1] // 2)
-        tx, tq, ts = x.c(), out.c(), scale.c()
-        self._check(_lib.hb_swiglu_quant(self._h, C.byref(tx), C.byref(tq), C.byref(ts)))
+        self._check(_lib.hb_swiglu_quant(self._h, x.addr(), out.addr(), scale.addr()))
         return out, scale
 
     def matmul_scaled(self, A: Tensor, a_scale: Tensor, B: Tensor, b_scale: Tensor, out: Optional[Tensor] = None,
@@ -367,14 +373,17 @@ class Context:
         """out[M,N] bf16 = epilogue(A @ B) of two quantised matrices: A [M,K] with a scale per row
         and 128 k, B [K,N] the `.T` of a weight matrix quantised in 128 x 128 blocks and b_scale
         the `.T` of its scales.  `weights` as for :meth:`matmul`."""
-        M, N = A.shape[0], B.shape[1]
         if out is None:
+            M, N = A.shape[0], B.shape[1]
             out = self.empty((M, N // 2 if epilogue == HB_EPI_SWIGLU else N), HB_BF16)
-        opts = _capi.hb_matmul_opts(epilogue | (_capi.HB_MATMUL_WEIGHTS_B if weights else 0), -1,
-                                    residual.ptr if residual else None, residual.stride[0] if residual else 0)
-        ta, tas, tb, tbs, tc = A.c(), a_scale.c(), B.c(), b_scale.c(), out.c()
-        self._check(_lib.hb_matmul_scaled(self._h, C.byref(ta), C.byref(tas), C.byref(tb), C.byref(tbs), C.byref(tc),
-                                          C.byref(opts)))
+        flags = epilogue | (_capi.HB_MATMUL_WEIGHTS_B if weights else 0)
+        opts = _OPTS.get(flags) if residual is None else None
+        if opts is None:
+            opts = _capi.hb_matmul_opts(flags, -1, residual.ptr if residual is not None else None,
+                                        residual.stride[0] if residual is not None else 0)
+            if residual is None:
+                _OPTS[flags] = opts
+        self._check(_lib.hb_matmul_scaled(self._h, A.addr(), a_scale.addr(), B.addr(), b_scale.addr(), out.addr(), C.addressof(opts)))
         return out
 
     # -- collective node ------------------------------------------------------------
