@@ -372,7 +372,8 @@ class Context:
                       epilogue: int = HB_EPI_NONE, residual: Optional[Tensor] = None, weights: bool = False) -> Tensor:
         """out[M,N] bf16 = epilogue(A @ B) of two quantised matrices: A [M,K] with a scale per row
         and 128 k, B [K,N] the `.T` of a weight matrix quantised in 128 x 128 blocks and b_scale
-        the `.T` of its scales.  `weights` as for :meth:`matmul`."""
+        the `.T` of its scales.  `weights` as for :meth:`matmul` (not for a B that a call still
+        in flight quantises)."""
         if out is None:
             M, N = A.shape[0], B.shape[1]
             out = self.empty((M, N // 2 if epilogue == HB_EPI_SWIGLU else N), HB_BF16)

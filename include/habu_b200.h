@@ -250,7 +250,9 @@ hb_status hb_argmax(hb_ctx* ctx, const void* x, int32_t* out, int64_t rows, int6
  *                      a_scale * b_scale and added in fp32; C is rounded once.  A and B need
  *                      16-byte aligned bases and row pitches that are multiples of 16; M, N and K
  *                      are free.  `opts` as for hb_matmul (epilogues and HB_MATMUL_WEIGHTS_B;
- *                      config_id must be -1); a residual must not overlap C.
+ *                      config_id must be -1); a residual must not overlap C.  The flag also covers
+ *                      b_scale; a product right behind the hb_quantize that makes its B goes
+ *                      without it, or behind an hb_sync.
  * None of them uses scratch or counters in device memory, and each adds up in a fixed order: equal
  * inputs give equal bits, and calls may overlap on the GPU. */
 hb_status hb_quantize(hb_ctx* ctx, const hb_tensor* x, hb_tensor* q, hb_tensor* scale, int32_t block_rows);
