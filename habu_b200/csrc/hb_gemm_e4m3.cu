@@ -113,25 +113,34 @@ constexpr uint32_t umma_idesc_e4m3(int m, int n) {
 // umma_desc_k_sw128), in two words: the low one carries the address and moves by plain addition.
 constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 __device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
-// One k-block: four MMAs of K = 32, the first of them overwriting D.  Executed by a whole converged
-// warp -- one thread issues -- so that the operands stay in uniform registers; a loop inside a
-// one-thread branch has to move every operand there and took some 500 clocks per k-block.
-template <int CTA_GROUP>
-__device__ __forceinline__ void umma_kblock(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
-#define HB_UMMA(GROUP, K, ACC)                                                                                            \
+// One step of K = 32 (number STEP of a k-block; the first overwrites D).
+#define HB_UMMA(GROUP, D, A_LO, B_LO, STEP)                                                                               \
   asm volatile(                                                                                                           \
       "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t" \
-      "tcgen05.mma.cta_group::" #GROUP ".kind::f8f6f4 [%0], da, db, %4, p;\n\t}\n" ::"r"(d_tmem),                          \
-      "r"(a_lo + (K) * (UMMA_K >> 4)), "r"(b_lo + (K) * (UMMA_K >> 4)), "r"(DESC_HI), "r"(idesc), "n"(ACC)                  \
+      "tcgen05.mma.cta_group::" #GROUP ".kind::f8f6f4 [%0], da, db, %4, p;\n\t}\n" ::"r"(D),                              \
+      "r"((A_LO) + (STEP) * (UMMA_K >> 4)), "r"((B_LO) + (STEP) * (UMMA_K >> 4)), "r"(DESC_HI), "r"(idesc), "n"((STEP) > 0)   \
       : "memory")
+static_assert(KB / UMMA_K == 4, "four steps");
+// One k-block.  Executed by a whole converged warp -- one thread issues -- so that the operands stay in uniform
+// registers; a loop inside a one-thread branch has to move every operand there and took some 500 clocks per
+// k-block.
+template <int CTA_GROUP>
+__device__ __forceinline__ void umma_kblock(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   if constexpr (CTA_GROUP == 1) {
-    HB_UMMA(1, 0, 0); HB_UMMA(1, 1, 1); HB_UMMA(1, 2, 1); HB_UMMA(1, 3, 1);
+    HB_UMMA(1, d, a_lo, b_lo, 0); HB_UMMA(1, d, a_lo, b_lo, 1); HB_UMMA(1, d, a_lo, b_lo, 2); HB_UMMA(1, d, a_lo, b_lo, 3);
   } else {
-    HB_UMMA(2, 0, 0); HB_UMMA(2, 1, 1); HB_UMMA(2, 2, 1); HB_UMMA(2, 3, 1);
+    HB_UMMA(2, d, a_lo, b_lo, 0); HB_UMMA(2, d, a_lo, b_lo, 1); HB_UMMA(2, d, a_lo, b_lo, 2); HB_UMMA(2, d, a_lo, b_lo, 3);
   }
-#undef HB_UMMA
-  static_assert(KB / UMMA_K == 4, "four steps");
 }
+// Two k-blocks for two slots, their steps in turn: with as few columns as A has rows there, an MMA waits longer
+// for the one before it on the same sums than it takes.
+__device__ __forceinline__ void umma_two(uint32_t d0, uint32_t a0, uint32_t b0, uint32_t d1, uint32_t a1, uint32_t b1, uint32_t idesc) {
+  HB_UMMA(1, d0, a0, b0, 0); HB_UMMA(1, d1, a1, b1, 0);
+  HB_UMMA(1, d0, a0, b0, 1); HB_UMMA(1, d1, a1, b1, 1);
+  HB_UMMA(1, d0, a0, b0, 2); HB_UMMA(1, d1, a1, b1, 2);
+  HB_UMMA(1, d0, a0, b0, 3); HB_UMMA(1, d1, a1, b1, 3);
+}
+#undef HB_UMMA
 // Two sums at once: acc += t * f.  Volatile like the tensor-memory load and the wait for it, so that it stays behind both.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t t0, uint32_t t1, uint64_t f) {
   asm volatile("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}" : "+l"(acc) : "r"(t0), "r"(t1), "l"(f));
@@ -784,8 +793,8 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // practice, and there is no scratch and no counter in global memory that launches could share.
 // With HB_MATMUL_WEIGHTS_B a CTA fills its ring with B before the kernel in front has finished
 // (programmatic dependent launch); what depends on that kernel comes after the wait.
-// 16 x 28672 x 4096 24.0 us, 16 x 128256 x 4096 80.7 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 8.7 us,
-// 64 x 28672 x 4096 31.6 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
+// 16 x 28672 x 4096 23.2 us, 16 x 128256 x 4096 80.9 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 8.3 us,
+// 64 x 28672 x 4096 30.3 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
 // launch are not it (start, the first bytes, the last sums; a second CTA on the SM would cover them, but
 // of kernels that allocate tensor memory the occupancy query admits one).  Measured and not taken: equal
 // units for all CTAs and partial sums in global memory (28 us for 16 x 28672 x 4096).
@@ -810,6 +819,9 @@ struct FewParams {
 template <int MP>
 struct FewLayout {
   static constexpr int A_BYTES = MP * KB, B_BYTES = SLAB * KB;
+  // Units that share a barrier.  Two for few columns: their MMAs run in turn (below), and the sums wait once
+  // for both.  With 64 it is slower (64 x 28672 x 4096 33.5 us, one by one 31.5).
+  static constexpr int GROUP = MP <= 32 ? 2 : 1, GROUPS = FEW_SLOTS / GROUP;
   static constexpr int MAX_CLUSTER = MP <= 16 ? 6 : 4;                    // the sums received have to fit beside the ring
   static constexpr uint32_t TMEM_COLS = FEW_SLOTS * MP;                   // 128, 256 or 512
   static constexpr int F_BYTES = FEW_SLOTS * MP * 4;                      // factors: [slot][MP] fp32
@@ -821,8 +833,8 @@ struct FewLayout {
   static constexpr int OFF_F = OFF_A + STAGES * A_BYTES;
   static constexpr int OFF_X = OFF_F + F_BYTES;
   static constexpr int OFF_W = OFF_X + X_BYTES;
-  static constexpr int OFF_BAR = OFF_W + W_BYTES;      // full, empty per stage; tfull, tempty, ffull per slot; xfull per warp
-  static constexpr int OFF_TMEM_PTR = OFF_BAR + (2 * STAGES + 3 * FEW_SLOTS + 4) * 8;
+  static constexpr int OFF_BAR = OFF_W + W_BYTES;      // full, empty per stage; tfull, tempty per group; xfull per warp
+  static constexpr int OFF_TMEM_PTR = OFF_BAR + (2 * STAGES + 2 * GROUPS + 4) * 8;
   static constexpr int OFF_ABORT = OFF_TMEM_PTR + 4;
   static constexpr int DYN_BYTES = OFF_ABORT + 4 + 1024;
   static_assert(DYN_BYTES <= 227 * 1024 && STAGES >= 4, "ring does not fit shared memory");
@@ -841,9 +853,8 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
   const uint32_t bar_full = smem_base + L::OFF_BAR;
   const uint32_t bar_empty = bar_full + L::STAGES * 8;
   const uint32_t bar_tfull = bar_empty + L::STAGES * 8;
-  const uint32_t bar_tempty = bar_tfull + FEW_SLOTS * 8;
-  const uint32_t bar_ffull = bar_tempty + FEW_SLOTS * 8;
-  const uint32_t bar_xfull = bar_ffull + FEW_SLOTS * 8;
+  const uint32_t bar_tempty = bar_tfull + L::GROUPS * 8;
+  const uint32_t bar_xfull = bar_tempty + L::GROUPS * 8;
   volatile uint32_t* tmem_ptr_smem = reinterpret_cast<volatile uint32_t*>(smem + L::OFF_TMEM_PTR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_ABORT);
 
@@ -880,10 +891,9 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
         mbar_init(bar_full + s * 8, 1);
         mbar_init(bar_empty + s * 8, 1);
       }
-      for (int a = 0; a < FEW_SLOTS; ++a) {
-        mbar_init(bar_tfull + a * 8, 1);
+      for (int a = 0; a < L::GROUPS; ++a) {
+        mbar_init(bar_tfull + a * 8, 2);         // the sums of the MMA, and the factors
         mbar_init(bar_tempty + a * 8, 4);
-        mbar_init(bar_ffull + a * 8, 1);
       }
       for (int w = 0; w < 4; ++w) mbar_init(bar_xfull + w * 8, max(senders, 1));
       mbar_fence_init();
@@ -944,23 +954,39 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     __syncwarp();
     constexpr uint32_t idesc = umma_idesc_e4m3(SLAB, MP);
     const uint32_t a_lo = desc_lo(sA), b_lo = desc_lo(sB);
-    int s = 0, slot = 0;
-    uint32_t phase = 0, slot_phase = 0;
+    int s = 0;
+    uint32_t phase = 0;
     bool ok = true;
-    for (int64_t u = 0; u < units; ++u) {
-      if (!mbar_wait(bar_full + s * 8, phase, abort_flag) || !mbar_wait(bar_tempty + slot * 8, slot_phase ^ 1, abort_flag)) {
+    for (int u = 0; u < units; u += L::GROUP) {
+      const int slot = u % FEW_SLOTS, group = slot / L::GROUP;
+      const bool both = L::GROUP == 2 && u + 1 < units;
+      const int s2 = s + 1 == L::STAGES ? 0 : s + 1;         // the next stage
+      const uint32_t phase2 = s2 ? phase : phase ^ 1;
+      if (!mbar_wait(bar_tempty + group * 8, (u / FEW_SLOTS & 1) ^ 1, abort_flag) || !mbar_wait(bar_full + s * 8, phase, abort_flag) ||
+          (both && !mbar_wait(bar_full + s2 * 8, phase2, abort_flag))) {
         ok = false;
         break;
       }
       tc_fence_after();
+      const uint32_t d = tmem_base + slot * MP, a0 = b_lo + s * (L::B_BYTES >> 4), b0 = a_lo + s * (L::A_BYTES >> 4);
+      const uint32_t a1 = b_lo + s2 * (L::B_BYTES >> 4), b1 = a_lo + s2 * (L::A_BYTES >> 4);
       if (elect_one()) {
-        umma_kblock<1>(tmem_base + slot * MP, b_lo + s * (L::B_BYTES >> 4), a_lo + s * (L::A_BYTES >> 4), idesc);
-        umma_commit<1>(bar_tfull + slot * 8);
-        umma_commit<1>(bar_empty + s * 8);
+        if (both) {
+          umma_two(d, a0, b0, d + MP, a1, b1, idesc);
+          umma_commit<1>(bar_empty + s * 8);
+          umma_commit<1>(bar_empty + s2 * 8);
+        } else {
+          umma_kblock<1>(d, a0, b0, idesc);
+          umma_commit<1>(bar_empty + s * 8);
+        }
+        umma_commit<1>(bar_tfull + group * 8);
       }
       __syncwarp();
-      if (++s == L::STAGES) { s = 0; phase ^= 1; }
-      if (++slot == FEW_SLOTS) { slot = 0; slot_phase ^= 1; }
+      s = s2;
+      phase = phase2;
+      if (both) {
+        if (++s == L::STAGES) { s = 0; phase ^= 1; }
+      }
     }
     if (!ok && lane == 0) report_timeout(p.status, 12);
   } else if (warp == 6) {
@@ -993,16 +1019,18 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     for (int j = 0; j < AHEAD; ++j) fetch_a(fa[j], first_kb[j]);
     uint32_t slot_phase = 0;
     bool ok = true;
-    for (int64_t u = 0; u < units && ok; u += AHEAD, slot_phase ^= 1) {
+    for (int u = 0; u < units && ok; u += AHEAD, slot_phase ^= 1) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         if (u + j < units && ok) {
-          ok = mbar_wait(bar_tempty + j * 8, slot_phase ^ 1, abort_flag);
+          if (j % L::GROUP == 0) ok = mbar_wait(bar_tempty + j / L::GROUP * 8, slot_phase ^ 1, abort_flag);
 #pragma unroll
           for (int i = 0; i < PER; ++i)
             if (lane + 32 * i < MP) factors[j * MP + lane + 32 * i] = fa[j][i] * fb[j];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_ffull + j * 8);
+          if (j % L::GROUP == L::GROUP - 1 || u + j + 1 == units) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_tfull + j / L::GROUP * 8);
+          }
           fb[j] = p.sb[slab * p.sb_n + kb * p.sb_k];
           fetch_a(fa[j], kb);
           next();
@@ -1018,8 +1046,6 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     const uint32_t x_mine = smem_base + L::OFF_X + r * 4;
     const float* x_local = reinterpret_cast<const float*>(smem + L::OFF_X) + r;
     float* w_local = reinterpret_cast<float*>(smem + L::OFF_W) + r;
-    int slot = 0;
-    uint32_t slot_phase = 0;
     bool ok = true;
     grid_dependency_wait();                      // C may still be in use by the kernel in front
     int slab = slab0, kb = kb0;
@@ -1028,26 +1054,43 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
       uint64_t acc[MP / 2];
 #pragma unroll
       for (int i = 0; i < MP / 2; ++i) acc[i] = 0;
-      for (int i = 0; i < nkb; ++i) {
-        ok = mbar_wait(bar_ffull + slot * 8, slot_phase, abort_flag) && mbar_wait(bar_tfull + slot * 8, slot_phase, abort_flag);
+      // a group's two slots at once where both belong to this slab
+      for (int i = 0; i < nkb;) {
+        const int at = static_cast<int>(u - u_begin) + i, slot = at % FEW_SLOTS;
+        const bool both = L::GROUP == 2 && slot % 2 == 0 && i + 1 < nkb;
+        ok = mbar_wait(bar_tfull + slot / L::GROUP * 8, at / FEW_SLOTS & 1, abort_flag);
         if (!ok) break;
         tc_fence_after();
+        auto add = [&](const uint32_t (&v)[MP / 16][16], int which) {
+          const float4* f4 = reinterpret_cast<const float4*>(factors + which * MP);
+#pragma unroll
+          for (int c = 0; c < MP / 4; ++c) {
+            const float4 f = f4[c];
+            const uint32_t* t = &v[c / 4][c % 4 * 4];
+            fma2(acc[2 * c], t[0], t[1], pack2(f.x, f.y));
+            fma2(acc[2 * c + 1], t[2], t[3], pack2(f.z, f.w));
+          }
+        };
         uint32_t v[MP / 16][16];
 #pragma unroll
         for (int c = 0; c < MP / 16; ++c) tmem_ld_32x16(t_mine + slot * MP + c * 16, v[c]);
-        tmem_wait_ld();
-        const float4* f4 = reinterpret_cast<const float4*>(factors + slot * MP);
+        if (both) {
+          uint32_t w[MP / 16][16];
 #pragma unroll
-        for (int c = 0; c < MP / 4; ++c) {
-          const float4 f = f4[c];
-          const uint32_t* t = &v[c / 4][c % 4 * 4];
-          fma2(acc[2 * c], t[0], t[1], pack2(f.x, f.y));
-          fma2(acc[2 * c + 1], t[2], t[3], pack2(f.z, f.w));
+          for (int c = 0; c < MP / 16; ++c) tmem_ld_32x16(t_mine + (slot + 1) * MP + c * 16, w[c]);
+          tmem_wait_ld();
+          add(v, slot);
+          add(w, slot + 1);
+        } else {
+          tmem_wait_ld();
+          add(v, slot);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_tempty + slot * 8);    // sums and factors are in registers
-        if (++slot == FEW_SLOTS) { slot = 0; slot_phase ^= 1; }
+        i += both ? 2 : 1;
+        if (both || slot % L::GROUP == L::GROUP - 1) {   // the group's sums and factors are in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_tempty + slot / L::GROUP * 8);
+        }
       }
       if (!ok) break;
       if (kb > 0) {
