@@ -793,7 +793,7 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // practice, and there is no scratch and no counter in global memory that launches could share.
 // With HB_MATMUL_WEIGHTS_B a CTA fills its ring with B before the kernel in front has finished
 // (programmatic dependent launch); what depends on that kernel comes after the wait.
-// 16 x 28672 x 4096 23.2 us, 16 x 128256 x 4096 80.9 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 8.3 us,
+// 16 x 28672 x 4096 22.6 us, 16 x 128256 x 4096 80.9 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 8.0 us,
 // 64 x 28672 x 4096 30.3 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
 // launch are not it (start, the first bytes, the last sums; a second CTA on the SM would cover them, but
 // of kernels that allocate tensor memory the occupancy query admits one).  Measured and not taken: equal
@@ -1155,9 +1155,10 @@ hb_matmul_scaled_few_kernel(const __grid_constant__ CUtensorMap tmA, const __gri
     if (!ok && lane == 0) report_timeout(p.status, 13);
   }
 
-  // no CTA may leave while a partner can still write to its shared memory
+  // no CTA may leave while a partner can still write to its shared memory (leaving one by one was also slower
+  // behind each other, 16 x 28672 x 4096 32.7 for 24.0 us: the next launch's clusters then find SMs in pieces)
   tc_fence_before();
-  cluster_sync();
+  if (S > 1) cluster_sync(); else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<1>(tmem_base, L::TMEM_COLS);
@@ -1211,12 +1212,18 @@ hb_status launch_few(hb_ctx* ctx, const ScaledArgs& g) {
   p.epilogue = g.epilogue;
   p.b_is_weights = g.b_is_weights;
   p.status = ctx->d_status;
-  // k-blocks that the busiest CTA streams
+  // CTAs of a cluster, by the longer of two times in microseconds: the busiest CTA's units at the rate of their
+  // MMAs, and the bytes at the rate of HBM, which takes about 120 CTAs.  Measured (M = 16, K = 4096; clusters of 1, 2, 3,
+  // 4, 6):  2048 columns 10.8 / 7.9 / 7.1 / 6.3 / 6.8     6144: 11.0 / 9.1 / 10.6 / 9.1 / 9.2
+  //   12288: 13.0 / 12.1 / 13.0 / 13.3 / 13.3   20480: 22.2 / 19.7 / 18.6 / 18.1 / 18.4   28672: 22.6 / 22.6 / 23.1 / 22.6 / 22.8
+  //   4096, K = 14336: 32.1 / 19.1 / 16.0 / 14.6 / 15.1; the choice is 1.6 % off the best on average, 9 % at most
+  const double unit = MP <= 32 ? 0.23 : 0.30, bytes = (double)(g.N + g.M) * g.K / 6.5e6;
   double best = 0;
   for (int c = 1; c <= L::MAX_CLUSTER && c <= p.num_kb; ++c) {
-    if (most[c] < 1) continue;
-    const int64_t at_once = most[c], clusters = p.slabs < at_once ? p.slabs : at_once;
-    const double cost = (double)((p.slabs + clusters - 1) / clusters) * p.num_kb / c;
+    const int at_once = most[c], clusters = p.slabs < at_once ? p.slabs : at_once;
+    if (clusters < 1) continue;
+    const double units = (double)((p.slabs + clusters - 1) / clusters) * p.num_kb / c, share = clusters * c / 120.0;
+    const double stream = share < 1 ? bytes / share : bytes, cost = units * unit > stream ? units * unit : stream;
     if (p.cluster == 0 || cost < best) { best = cost; p.cluster = c; }
   }
   const int at_once = most[p.cluster], clusters = p.slabs < at_once ? p.slabs : at_once;
