@@ -793,8 +793,8 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // practice, and there is no scratch and no counter in global memory that launches could share.
 // With HB_MATMUL_WEIGHTS_B a CTA fills its ring with B before the kernel in front has finished
 // (programmatic dependent launch); what depends on that kernel comes after the wait.
-// 16 x 28672 x 4096 22.6 us, 16 x 128256 x 4096 80.9 us (6.5 TB/s, 99 % of a copy), 1 x 6144 x 4096 8.0 us,
-// 64 x 28672 x 4096 30.3 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
+// 16 x 28672 x 4096 22.6 us, 16 x 128256 x 4096 79.1 us (6.6 TB/s, as fast as a copy), 1 x 6144 x 4096 8.0 us,
+// 64 x 28672 x 4096 30.4 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
 // launch are not it (start, the first bytes, the last sums; a second CTA on the SM would cover them, but
 // of kernels that allocate tensor memory the occupancy query admits one).  Measured and not taken: equal
 // units for all CTAs and partial sums in global memory (28 us for 16 x 28672 x 4096).
