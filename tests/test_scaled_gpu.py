@@ -631,3 +631,37 @@ def test_gelu_epilogue_over_its_range(ctx, step, K):
         s[0, 0] = value
         c = oracle.from_bf16_bits(ctx.download(ctx.matmul_scaled(A, ctx.upload(s), B.T, SB.T, epilogue=hb.HB_EPI_GELU)))
         assert np.isnan(c[0]).all() if np.isnan(value) else (c[0] == np.inf).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(4100, 1158, 144), (2050, 4614, 128), (200, 38402, 128), (600, 1414, 256)])
+@pytest.mark.parametrize("epi", [hb.HB_EPI_NONE, hb.HB_EPI_SWIGLU, hb.HB_EPI_RESIDUAL])
+def test_matmul_scaled_tiles_at_odd_addresses(ctx, M, N, K, epi):
+    """Whole tiles whose rows start on every multiple of two bytes, from one row to the next and from one
+    start to another, for every width that a warp writes; the edges beside them stay as they were."""
+    rng = np.random.default_rng(N)
+    ab, sa, av = qr.operands(rng, M, K, 1)
+    bb, sb, bv = qr.operands(rng, N, K, 128)
+    A, SA = _upload_pair(ctx, ab, sa)
+    B, SB = _upload_pair(ctx, bb, sb)
+    acc = av @ bv.T
+    size = np.abs(av) @ np.abs(bv).T
+    if epi == hb.HB_EPI_SWIGLU:
+        base, slope = qr.silu(acc[:, 0::2]) * acc[:, 1::2], None
+        # |silu'| < 1.1: the two factors' errors, each (K + 8) 2^-23 of its sums; silu itself 2^-20
+        e = (K + 8) * 2.0 ** -23
+        loose = 1.1 * np.abs(acc[:, 1::2]) * size[:, 0::2] * e + np.abs(acc[:, 0::2]) * size[:, 1::2] * e + np.abs(base) * 2.0 ** -19
+    else:
+        base, loose = acc, size * (K + 8) * 2.0 ** -23
+    out = base.shape[1]
+    for pad, shift in ((1, 0), (0, 1), (3, 2), (2, 3), (5, 7)):
+        c = COut(ctx, M, out, pad, shift)
+        res, want = None, base
+        if epi == hb.HB_EPI_RESIDUAL:
+            r, rb = _bf16(rng, (M, out + pad))
+            rbuf = ctx.upload(np.concatenate([np.full(shift, 0x7FC0, np.uint16), rb.reshape(-1)]))
+            res = ctx.wrap(rbuf.ptr + 2 * shift, (M, out), hb.HB_BF16, (out + pad, 1))
+            want = base + r[:, :out]
+        ctx.matmul_scaled(A, SA, B.T, SB.T, c.t, epilogue=epi, residual=res)
+        got = c.finish()
+        assert np.all(np.abs(got - want) <= np.abs(want) * (2.0 ** -8 + 2.0 ** -22) + loose + 1e-30), (pad, shift)
+    _free(ctx, A, SA, B, SB)
