@@ -783,9 +783,9 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // ------------------------------------------------------------------------------------
 // Few rows (M <= 64): bound by reading B once.  The operands change places -- a slab of 128 rows of B
 // is the M side of the MMA, the rows of A, padded to 16, 32 or 64 by TMA's zero fill, its N side.
-// A cluster of S CTAs owns whole slabs and cuts their (slab, k-block) units into S contiguous ranges of
-// the same length, one per CTA, so that every SM streams the same number of bytes.  A finished k-block
-// goes to one of eight tensor-memory slots; a thread holds one column of C (one row of the slab) for
+// A CTA, or a cluster of S, owns whole slabs; a cluster cuts their (slab, k-block) units into S contiguous
+// ranges of the same length, one per CTA, so that its SMs stream the same number of bytes.  A finished
+// k-block goes to one of eight tensor-memory slots; a thread holds one column of C (one row of the slab) for
 // all rows of A, and the factors a_scale * b_scale of a k-block come through shared memory from a warp
 // that runs ahead.  Where a range starts inside a slab, its sums go to the CTA that started the slab, over
 // distributed shared memory, as the first thing that a CTA finishes; the starter comes to that slab
@@ -796,8 +796,10 @@ hb_status launch_tile_epi(hb_ctx* ctx, const ScaledArgs& g, int split) {
 // 16 x 28672 x 4096 22.6 us, 16 x 128256 x 4096 79.1 us (6.6 TB/s, as fast as a copy), 1 x 6144 x 4096 8.0 us,
 // 64 x 28672 x 4096 30.4 us: the stream itself runs at 6 to 7 TB/s, and about five microseconds of a
 // launch are not it (start, the first bytes, the last sums; a second CTA on the SM would cover them, but
-// of kernels that allocate tensor memory the occupancy query admits one).  Measured and not taken: equal
-// units for all CTAs and partial sums in global memory (28 us for 16 x 28672 x 4096).
+// of kernels that allocate tensor memory the occupancy query admits one).  A unit's MMAs take 0.25 us, as
+// long for a lower slab.  Measured and not taken: equal units for all CTAs and partial sums in global memory
+// (28 us for 16 x 28672 x 4096); slabs of as many rows as give every CTA the same (no gain, above 10 us for
+// 1 x 6144 x 4096); A loaded by a warp of its own, and scales fetched further ahead (no change).
 // ------------------------------------------------------------------------------------
 constexpr int FEW_MAX_M = 64;
 constexpr int FEW_THREADS = 224;                 // TMA, MMA, four warps of sums, factors

@@ -35,7 +35,8 @@ __device__ __forceinline__ uint32_t f2_to_bf2(float a, float b) {
 // Two fp32 products, and two multiply-adds, in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   uint64_t d;
-  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\tmul.rn.f32x2 %0, x, y;\n\t}" : "=l"(d) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\tmul.rn.f32x2 %0, x, y;\n\t}"
+      : "=l"(d) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   float2 r;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(d));
   return r;
@@ -108,10 +109,12 @@ __device__ __forceinline__ uint2 pack8(const float (&y)[8], const Scale& z) {
 // With h = x * gain, y = h * r and max|y| = max|h| * r for the row's r = rsqrt(..): y / scale = h * 448 / max|h|
 // does not depend on the row's statistic.  So a vector is done with at once and no row stays in registers;
 // the scales come behind, for BATCH rows at a time: one barrier, and one thread per group adds up the
-// row's sum (a barrier per row, with one warp at the scales and the others waiting for it: a tenth slower).  Where y / scale is not that (the scale meets its floor, r or a maximum is not finite), that
+// row's sum (a barrier per row, with one warp at the scales and the others waiting for it, was a tenth
+// slower).  Where y / scale is not that (the scale meets its floor, r or a maximum is not finite), that
 // thread forms the group's q again, from y.
-// Bound by HBM with the residual: 8192 x 4096 37.8 us (6.2 TB/s, 95 % of a copy).  Without it 20.0 us (5.0 TB/s),
-// bound by its instructions (118 per warp and 256 values; 69 % of the issue slots taken); 16 x 4096 2.1 us.  With y in registers until the statistic was there, q formed from it: 37.9 and 26.5 us.
+// Bound by HBM with the residual: 8192 x 4096 37.8 us (6.2 TB/s, 95 % of a copy).  Without it 20.0 us
+// (5.0 TB/s), bound by its instructions (118 per warp and 256 values; 69 % of the issue slots taken);
+// 16 x 4096 2.1 us.  With y in registers until the statistic was there and q formed from it: 37.9 and 26.5 us.
 constexpr int RMS_MAX_COLS = 16384;
 
 struct NormParams {
@@ -203,7 +206,7 @@ __global__ void __launch_bounds__(THREADS) rmsnorm_quant_kernel(const NormParams
           }
           if (in && row < p.rows) reinterpret_cast<uint4*>(p.residual + row * p.ldr)[t + i * tpr] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        uint4 gv;
+        uint4 gv = {};
         if constexpr (!L::GAIN_IN_REGS) gv = mine[L::STAGES * L::PER_STAGE + i * THREADS];
         const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
         float2 part = make_float2(0.f, 0.f);
