@@ -665,3 +665,29 @@ def test_matmul_scaled_tiles_at_odd_addresses(ctx, M, N, K, epi):
         got = c.finish()
         assert np.all(np.abs(got - want) <= np.abs(want) * (2.0 ** -8 + 2.0 ** -22) + loose + 1e-30), (pad, shift)
     _free(ctx, A, SA, B, SB)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_fp32_rounds_once(ctx, block_rows):
+    """fp32 values a unit in the last place on either side of the points half-way between two e4m3 values, for
+    many scales: q is the nearest value of the quotient in 64 bits wherever that is not a tie itself."""
+    rng = np.random.default_rng(5)
+    rows, cols = 256, 256
+    x = rng.uniform(-1, 1, (rows, cols)).astype(np.float32)
+    top = rng.uniform(1, 2, (rows // block_rows, 2)).astype(np.float32)
+    tops = np.repeat(np.repeat(top, block_rows, 0), 128, 1).astype(np.float64)
+    vals = np.sort(qr.VALUES[:127])
+    half = (vals[1:] + vals[:-1]) / 2
+    pick = half[rng.integers(0, len(half), (rows, cols))] * tops / 448
+    x = np.nextafter(pick.astype(np.float32), np.where(rng.random((rows, cols)) < 0.5, np.float32(0), np.float32(9)), dtype=np.float32)
+    x = np.where(rng.random((rows, cols)) < 0.3, pick.astype(np.float32), x) * np.where(rng.random((rows, cols)) < 0.5, 1, -1).astype(np.float32)
+    for i in range(rows // block_rows):
+        for j in range(2):
+            x[i * block_rows, 128 * j] = top[i, j]
+    q, s = ctx.quantize(ctx.upload(x), block_rows=block_rows)
+    t = x.astype(np.float64) * 448 / tops                # (two roundings of 2^-53)
+    lower = np.searchsorted(half, np.abs(t))
+    tie = np.abs(np.abs(t) - half[np.minimum(lower, len(half) - 1)]) <= np.abs(t) * 2.0 ** -51
+    tie |= np.abs(np.abs(t) - half[np.maximum(lower - 1, 0)]) <= np.abs(t) * 2.0 ** -51
+    want = np.copysign(vals[lower], t)
+    assert np.array_equal(qr.decode(_pitched(ctx, q))[~tie], want[~tie]) and (~tie).mean() > 0.5
